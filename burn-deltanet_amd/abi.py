@@ -17,10 +17,10 @@ import torch
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libdeltanet_core.so"
 
-DN_F32, DN_BF16 = 0, 1
+DN_F32, DN_BF16, DN_F8 = 0, 1, 2
 DN_ALGO_AUTO, DN_ALGO_GENERIC, DN_ALGO_MFMA, DN_ALGO_MFMA_FUSED = 0, 1, 2, 3
 RECURRENT_MAX_K = 512  # dn_recurrent's head_k_dim limit (deltanet_core.h)
-DN_ACT_IDENTITY, DN_ACT_SILU, DN_ACT_RELU, DN_ACT_ELU_PLUS_ONE = 0, 1, 2, 3
+DN_ACT_IDENTITY, DN_ACT_SILU, DN_ACT_RELU, DN_ACT_ELU_PLUS_ONE, DN_ACT_GELU = 0, 1, 2, 3, 4
 DN_QKNORM_NONE, DN_QKNORM_L2, DN_QKNORM_SUM = 0, 1, 2
 DN_WRITE_FIXED, DN_WRITE_SCALAR, DN_WRITE_CHANNEL = 0, 1, 2
 FRONTEND_MAX_HEAD_DIM, FRONTEND_MAX_KERNEL = 256, 8
@@ -51,6 +51,10 @@ EXPORTS = [
     "dn_chunk_fwd_noalloc", "dn_unit_lower_inverse", "dn_block_step",
     "dn_chunk_fwd_out_norm", "dn_chunk_fwd_out_norm_workspace_bytes", "dn_wait_give_ups",
     "dn_frontend_chunk_fwd", "dn_frontend_chunk_fwd_workspace_bytes",
+    "dn_add_rms_norm", "dn_add_rms_norm_bwd", "dn_add_rms_norm_bwd_workspace_bytes",
+    "dn_linear", "dn_linear_workspace_bytes", "dn_linear_bwd", "dn_linear_bwd_workspace_bytes",
+    "dn_gated_ffn", "dn_gated_ffn_workspace_bytes", "dn_gated_ffn_bwd",
+    "dn_gated_ffn_bwd_workspace_bytes",
 ]
 NOALLOC_SCRATCH_BYTES = 64 << 20  # DN_NOALLOC_SCRATCH_BYTES (deltanet_core.h)
 
@@ -158,6 +162,74 @@ class TriArgs(ctypes.Structure):
     ]
 
 
+class AddRmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("x_stride", _i64), ("residual_stride", _i64),
+        ("sum_stride", _i64), ("out_stride", _i64), ("eps", _f64), ("dtype", _i32),
+        ("weight_dtype", _i32), ("out_dtype", _i32), ("x", _vp), ("residual", _vp),
+        ("weight", _vp), ("sum", _vp), ("out", _vp), ("scale", _vp),
+    ]
+
+
+class AddRmsNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("sum_stride", _i64), ("d_out_stride", _i64),
+        ("d_sum_stride", _i64), ("d_x_stride", _i64), ("eps", _f64), ("dtype", _i32),
+        ("weight_dtype", _i32), ("sum", _vp), ("weight", _vp), ("d_out", _vp), ("d_sum", _vp),
+        ("d_x", _vp), ("d_weight", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("in_dim", _i64), ("out_dim", _i64), ("x_stride", _i64),
+        ("weight_stride", _i64), ("residual_stride", _i64), ("out_stride", _i64),
+        ("preact_stride", _i64), ("dtype", _i32), ("out_dtype", _i32), ("activation", _i32),
+        ("x", _vp), ("weight", _vp), ("x_scale", _vp), ("weight_scale", _vp), ("bias", _vp),
+        ("residual", _vp), ("out", _vp), ("preact", _vp), ("workspace", _vp),
+        ("workspace_bytes", _sz),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("in_dim", _i64), ("out_dim", _i64), ("x_stride", _i64),
+        ("weight_stride", _i64), ("d_out_stride", _i64), ("preact_stride", _i64),
+        ("d_x_stride", _i64), ("dtype", _i32), ("activation", _i32), ("d_out", _vp), ("x", _vp),
+        ("weight", _vp), ("preact", _vp), ("d_x", _vp), ("d_weight", _vp), ("d_bias", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class GatedFfnArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("hidden", _i64), ("x_stride", _i64),
+        ("w_in_stride", _i64), ("w_down_stride", _i64), ("residual_stride", _i64),
+        ("out_stride", _i64), ("kept_stride", _i64), ("dtype", _i32), ("activation", _i32),
+        ("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("residual", _vp),
+        ("out", _vp), ("gate", _vp), ("up", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class GatedFfnBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("hidden", _i64), ("x_stride", _i64),
+        ("w_in_stride", _i64), ("w_down_stride", _i64), ("d_out_stride", _i64),
+        ("kept_stride", _i64), ("d_x_stride", _i64), ("dtype", _i32), ("activation", _i32),
+        ("d_out", _vp), ("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp),
+        ("gate", _vp), ("up", _vp), ("d_x", _vp), ("d_w_gate", _vp), ("d_w_up", _vp),
+        ("d_w_down", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+# The operators around the mixer: (entry, its argument struct, whether a
+# *_workspace_bytes entry goes with it).
+_LAYER = [
+    ("dn_add_rms_norm", AddRmsNormArgs, False), ("dn_add_rms_norm_bwd", AddRmsNormBwdArgs, True),
+    ("dn_linear", LinearArgs, True), ("dn_linear_bwd", LinearBwdArgs, True),
+    ("dn_gated_ffn", GatedFfnArgs, True), ("dn_gated_ffn_bwd", GatedFfnBwdArgs, True),
+]
+
 _LIB = None
 
 
@@ -212,6 +284,12 @@ def lib() -> ctypes.CDLL:
                                       ctypes.POINTER(ctypes.c_double),
                                       ctypes.POINTER(ctypes.c_int64)]
         L.dn_profile_read.restype = ctypes.c_int
+        for name, struct, sized in _LAYER:
+            getattr(L, name).argtypes = [ctypes.POINTER(struct), _vp]
+            getattr(L, name).restype = ctypes.c_int
+            if sized:
+                getattr(L, name + "_workspace_bytes").argtypes = [ctypes.POINTER(struct)]
+                getattr(L, name + "_workspace_bytes").restype = _sz
         L.dn_last_error.restype = ctypes.c_char_p
         L.dn_version.restype = ctypes.c_char_p
         _LIB = L

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "dn_common.hpp"
+#include "layer.hpp"
 
 namespace dn {
 namespace {
@@ -892,6 +893,264 @@ int dn_out_norm(const dn_out_norm_args* a, hipStream_t stream) {
   hipError_t e = launch_out_norm(*a, stream);
   if (e != hipSuccess) return hip_fail(e, "dn_out_norm launch");
   return DN_OK;
+}
+
+// --- the operators around the mixer ------------------------------------------
+
+namespace {
+
+// A [rows, dim] tensor: a pointer where there are rows, rows that do not
+// overlap. `what` names it in the message.
+int check_rows(const void* p, int64_t rows, int64_t dim, int64_t stride, const char* what) {
+  if (!p && rows > 0) return fail(DN_ERR_NULL, std::string(what) + " is NULL");
+  if (rows > 1 && (stride < dim || stride >= (int64_t(1) << 40)))
+    return fail(DN_ERR_SHAPE, std::string(what) + ": rows of " + std::to_string(dim) +
+                                  " values cannot be " + std::to_string(stride) + " apart");
+  return DN_OK;
+}
+// The same for a tensor that may be absent.
+int check_rows_opt(const void* p, int64_t rows, int64_t dim, int64_t stride, const char* what) {
+  return p ? check_rows(p, rows, dim, stride, what) : DN_OK;
+}
+
+int check_sizes(int64_t rows, std::initializer_list<int64_t> widths) {
+  if (rows < 0) return fail(DN_ERR_SHAPE, "rows must not be negative");
+  int64_t most = 1, product = 1;
+  for (const int64_t w : widths) {
+    if (w < 1) return fail(DN_ERR_SHAPE, "every width must be at least 1");
+    most = w > most ? w : most;
+    // A row's bytes and a weight's extent stay inside the kernels' 32-bit
+    // column arithmetic.
+    if (w > (int64_t(1) << 24)) return fail(DN_ERR_SHAPE, "tensor too large");
+    product *= w;
+    if (product >= (int64_t(1) << 40)) return fail(DN_ERR_SHAPE, "tensor too large");
+  }
+  if (rows > INT32_MAX - 512 || too_large({rows, most}, int64_t(1) << 40))
+    return fail(DN_ERR_SHAPE, "tensor too large");
+  return DN_OK;
+}
+
+int check_activation(int act) {
+  if (act != DN_ACT_IDENTITY && act != DN_ACT_SILU && act != DN_ACT_RELU && act != DN_ACT_GELU)
+    return fail(DN_ERR_SHAPE, "activation must be identity, SiLU, ReLU or GELU");
+  return DN_OK;
+}
+
+int workspace_for(size_t need, void* given, size_t given_bytes, hipStream_t stream, void** ws) {
+  *ws = given;
+  if (!need) return DN_OK;
+  if (given) {
+    if (given_bytes < need)
+      return fail(DN_ERR_WORKSPACE, "workspace too small: need " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(given) % 16)
+      return fail(DN_ERR_WORKSPACE, "the workspace must start at a 16-byte boundary");
+    return DN_OK;
+  }
+  const hipError_t e = pool_get(need, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "workspace allocation");
+}
+
+int check_norm_types(int32_t dtype, int32_t weight_dtype, double eps) {
+  if (!valid_dtype(dtype) || !valid_dtype(weight_dtype))
+    return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  if (!(eps >= 0.0)) return fail(DN_ERR_SHAPE, "eps must be a non-negative number");
+  return DN_OK;
+}
+
+int check_add_rms_norm_bwd(const dn_add_rms_norm_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim})) return rc;
+  if (int rc = check_norm_types(a->dtype, a->weight_dtype, a->eps)) return rc;
+  if (int rc = check_rows(a->sum, a->rows, a->dim, a->sum_stride, "sum")) return rc;
+  if (int rc = check_rows(a->d_out, a->rows, a->dim, a->d_out_stride, "d_out")) return rc;
+  if (int rc = check_rows_opt(a->d_sum, a->rows, a->dim, a->d_sum_stride, "d_sum")) return rc;
+  if (int rc = check_rows(a->d_x, a->rows, a->dim, a->d_x_stride, "d_x")) return rc;
+  if (!a->weight) return fail(DN_ERR_NULL, "weight is NULL");
+  return DN_OK;
+}
+
+int check_linear(const dn_linear_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->in_dim, a->out_dim})) return rc;
+  const bool f8in = a->dtype == DN_F8;
+  if ((!valid_dtype(a->dtype) && !f8in) || !valid_dtype(a->out_dtype))
+    return fail(DN_ERR_DTYPE, "dtype must be DN_F32, DN_BF16 or (operands) DN_F8");
+  if (!f8in && a->out_dtype != a->dtype)
+    return fail(DN_ERR_DTYPE, "out_dtype must be the operands' dtype");
+  if (int rc = check_activation(a->activation)) return rc;
+  if (int rc = check_rows(a->x, a->rows, a->in_dim, a->x_stride, "x")) return rc;
+  if (int rc = f8in ? check_rows(a->weight, a->out_dim, a->in_dim, a->weight_stride, "weight")
+                    : check_rows(a->weight, a->in_dim, a->out_dim, a->weight_stride, "weight"))
+    return rc;
+  if (int rc = check_rows_opt(a->residual, a->rows, a->out_dim, a->residual_stride, "residual"))
+    return rc;
+  if (int rc = check_rows(a->out, a->rows, a->out_dim, a->out_stride, "out")) return rc;
+  if (int rc = check_rows_opt(a->preact, a->rows, a->out_dim, a->preact_stride, "preact")) return rc;
+  if (f8in) {
+    if ((!a->x_scale && a->rows > 0) || !a->weight_scale)
+      return fail(DN_ERR_NULL, "8-bit operands need their scales");
+    const int64_t padded = (a->in_dim + 15) / 16 * 16;
+    const auto whole = [&](const void* p, int64_t stride) {
+      return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride >= padded;
+    };
+    if (!whole(a->x, a->x_stride) || !whole(a->weight, a->weight_stride))
+      return fail(DN_ERR_UNSUPPORTED, "8-bit rows must start at 16-byte boundaries and hold "
+                                      "zeros up to the next multiple of 16");
+  }
+  return DN_OK;
+}
+
+int check_linear_bwd(const dn_linear_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->in_dim, a->out_dim})) return rc;
+  if (!valid_dtype(a->dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  if (int rc = check_activation(a->activation)) return rc;
+  if (int rc = check_rows(a->d_out, a->rows, a->out_dim, a->d_out_stride, "d_out")) return rc;
+  if (a->d_weight)
+    if (int rc = check_rows(a->x, a->rows, a->in_dim, a->x_stride, "x")) return rc;
+  if (a->d_x) {
+    if (int rc = check_rows(a->weight, a->in_dim, a->out_dim, a->weight_stride, "weight")) return rc;
+    if (int rc = check_rows(a->d_x, a->rows, a->in_dim, a->d_x_stride, "d_x")) return rc;
+  }
+  if (a->activation != DN_ACT_IDENTITY)
+    return check_rows(a->preact, a->rows, a->out_dim, a->preact_stride, "preact");
+  return DN_OK;
+}
+
+int check_gated_ffn(const dn_gated_ffn_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim, a->hidden})) return rc;
+  if (!valid_dtype(a->dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  if (int rc = check_activation(a->activation)) return rc;
+  if (int rc = check_rows(a->x, a->rows, a->dim, a->x_stride, "x")) return rc;
+  if (int rc = check_rows(a->w_gate, a->dim, a->hidden, a->w_in_stride, "w_gate")) return rc;
+  if (int rc = check_rows(a->w_up, a->dim, a->hidden, a->w_in_stride, "w_up")) return rc;
+  if (int rc = check_rows(a->w_down, a->hidden, a->dim, a->w_down_stride, "w_down")) return rc;
+  if (int rc = check_rows_opt(a->residual, a->rows, a->dim, a->residual_stride, "residual"))
+    return rc;
+  if (int rc = check_rows(a->out, a->rows, a->dim, a->out_stride, "out")) return rc;
+  if (!a->gate != !a->up) return fail(DN_ERR_NULL, "gate and up are kept together");
+  if (int rc = check_rows_opt(a->gate, a->rows, a->hidden, a->kept_stride, "gate")) return rc;
+  return check_rows_opt(a->up, a->rows, a->hidden, a->kept_stride, "up");
+}
+
+int check_gated_ffn_bwd(const dn_gated_ffn_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim, a->hidden})) return rc;
+  if (!valid_dtype(a->dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  if (int rc = check_activation(a->activation)) return rc;
+  if (int rc = check_rows(a->d_out, a->rows, a->dim, a->d_out_stride, "d_out")) return rc;
+  if (int rc = check_rows(a->gate, a->rows, a->hidden, a->kept_stride, "gate")) return rc;
+  if (int rc = check_rows(a->up, a->rows, a->hidden, a->kept_stride, "up")) return rc;
+  if (int rc = check_rows(a->w_down, a->hidden, a->dim, a->w_down_stride, "w_down")) return rc;
+  if (!a->d_w_gate != !a->d_w_up)
+    return fail(DN_ERR_NULL, "d_w_gate and d_w_up are formed together");
+  if (a->d_x) {
+    if (int rc = check_rows(a->w_gate, a->dim, a->hidden, a->w_in_stride, "w_gate")) return rc;
+    if (int rc = check_rows(a->w_up, a->dim, a->hidden, a->w_in_stride, "w_up")) return rc;
+    if (int rc = check_rows(a->d_x, a->rows, a->dim, a->d_x_stride, "d_x")) return rc;
+  }
+  if (a->d_w_gate)
+    if (int rc = check_rows(a->x, a->rows, a->dim, a->x_stride, "x")) return rc;
+  return DN_OK;
+}
+
+}  // namespace
+
+int dn_add_rms_norm(const dn_add_rms_norm_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim})) return rc;
+  if (int rc = check_norm_types(a->dtype, a->weight_dtype, a->eps)) return rc;
+  if (a->out_dtype != a->dtype && a->out_dtype != DN_F8)
+    return fail(DN_ERR_DTYPE, "out_dtype must be dtype or DN_F8");
+  if (int rc = check_rows(a->x, a->rows, a->dim, a->x_stride, "x")) return rc;
+  if (int rc = check_rows_opt(a->residual, a->rows, a->dim, a->residual_stride, "residual"))
+    return rc;
+  if (int rc = check_rows_opt(a->sum, a->rows, a->dim, a->sum_stride, "sum")) return rc;
+  if (int rc = check_rows(a->out, a->rows, a->dim, a->out_stride, "out")) return rc;
+  if (!a->weight) return fail(DN_ERR_NULL, "weight is NULL");
+  if (a->out_dtype == DN_F8 && !a->scale && a->rows > 0)
+    return fail(DN_ERR_NULL, "an 8-bit output needs its scales");
+  if (a->rows == 0) return DN_OK;
+  const hipError_t e = launch_add_rms_norm(*a, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_add_rms_norm launch");
+}
+
+size_t dn_add_rms_norm_bwd_workspace_bytes(const dn_add_rms_norm_bwd_args* a) {
+  return check_add_rms_norm_bwd(a) ? 0 : add_rms_norm_bwd_workspace(*a);
+}
+
+int dn_add_rms_norm_bwd(const dn_add_rms_norm_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_add_rms_norm_bwd(a)) return rc;
+  if (a->rows == 0 && !a->d_weight) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(add_rms_norm_bwd_workspace(*a), a->workspace, a->workspace_bytes,
+                             stream, &ws))
+    return rc;
+  const hipError_t e = launch_add_rms_norm_bwd(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_add_rms_norm_bwd launch");
+}
+
+size_t dn_linear_workspace_bytes(const dn_linear_args* a) {
+  return check_linear(a) || a->rows == 0 ? 0 : linear_workspace(*a);
+}
+
+int dn_linear(const dn_linear_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_linear(a)) return rc;
+  if (a->rows == 0) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(linear_workspace(*a), a->workspace, a->workspace_bytes, stream, &ws))
+    return rc;
+  const hipError_t e = launch_linear(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_linear launch");
+}
+
+size_t dn_linear_bwd_workspace_bytes(const dn_linear_bwd_args* a) {
+  return check_linear_bwd(a) ? 0 : linear_bwd_workspace(*a);
+}
+
+int dn_linear_bwd(const dn_linear_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_linear_bwd(a)) return rc;
+  void* ws = nullptr;
+  if (int rc = workspace_for(linear_bwd_workspace(*a), a->workspace, a->workspace_bytes, stream,
+                             &ws))
+    return rc;
+  const hipError_t e = launch_linear_bwd(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_linear_bwd launch");
+}
+
+size_t dn_gated_ffn_workspace_bytes(const dn_gated_ffn_args* a) {
+  return check_gated_ffn(a) || a->rows == 0 ? 0 : gated_ffn_workspace(*a);
+}
+
+int dn_gated_ffn(const dn_gated_ffn_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_gated_ffn(a)) return rc;
+  if (a->rows == 0) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(gated_ffn_workspace(*a), a->workspace, a->workspace_bytes, stream, &ws))
+    return rc;
+  const hipError_t e = launch_gated_ffn(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_gated_ffn launch");
+}
+
+size_t dn_gated_ffn_bwd_workspace_bytes(const dn_gated_ffn_bwd_args* a) {
+  return check_gated_ffn_bwd(a) ? 0 : gated_ffn_bwd_workspace(*a);
+}
+
+int dn_gated_ffn_bwd(const dn_gated_ffn_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_gated_ffn_bwd(a)) return rc;
+  void* ws = nullptr;
+  if (int rc = workspace_for(gated_ffn_bwd_workspace(*a), a->workspace, a->workspace_bytes, stream,
+                             &ws))
+    return rc;
+  const hipError_t e = launch_gated_ffn_bwd(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_gated_ffn_bwd launch");
 }
 
 int dn_block_step(const dn_block_step_args* a, hipStream_t stream) {

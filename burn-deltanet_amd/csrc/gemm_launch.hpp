@@ -1,0 +1,28 @@
+// Launches of the tile kernel for one operand type (included by the files
+// that hold its instantiations).
+#pragma once
+
+#include "gemm.hpp"
+#include "layer.hpp"
+
+namespace dn {
+namespace {
+
+template <class T, class TO, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, int EPI,
+          bool STAGED>
+hipError_t gemm_go(const GemmArgs& g, hipStream_t stream) {
+  const auto fn = gemm_kernel<T, TO, ACOL, BCOL, BM, BN, WM, WN, EPI, STAGED>;
+  const int64_t total = int64_t(g.tiles_m) * g.tiles_n * g.npair * g.split;
+  hipLaunchKernelGGL(fn, dim3(unsigned(total)), dim3(64 * WM * WN), 0, stream, g);
+  return hipGetLastError();
+}
+
+template <class T, class TO, bool ACOL, bool BCOL, int EPI, bool STAGED>
+hipError_t gemm_tile(const GemmArgs& g, GemmTile tile, hipStream_t stream) {
+  if (tile == kTile256)
+    return gemm_go<T, TO, ACOL, BCOL, 256, 256, 2, 4, EPI, STAGED>(g, stream);
+  return gemm_go<T, TO, ACOL, BCOL, 128, 128, 2, 2, EPI, STAGED>(g, stream);
+}
+
+}  // namespace
+}  // namespace dn

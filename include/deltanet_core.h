@@ -55,6 +55,7 @@ extern "C" {
 typedef enum {
   DN_F32 = 0,
   DN_BF16 = 1,
+  DN_F8 = 2, /* e4m3 (finite range +-448): dn_add_rms_norm's output and dn_linear's operands */
 } dn_dtype;
 
 /* Which kernels run dn_chunk_fwd / dn_chunk_bwd. AUTO picks the MFMA path
@@ -223,8 +224,9 @@ int dn_recurrent(const dn_recurrent_args *args, hipStream_t stream);
 typedef enum {
   DN_ACT_IDENTITY = 0,
   DN_ACT_SILU = 1,
-  DN_ACT_RELU = 2,          /* q/k activation only */
-  DN_ACT_ELU_PLUS_ONE = 3   /* q/k activation only */
+  DN_ACT_RELU = 2,          /* q/k activation, dn_linear, dn_gated_ffn */
+  DN_ACT_ELU_PLUS_ONE = 3,  /* q/k activation only */
+  DN_ACT_GELU = 4           /* dn_linear and dn_gated_ffn only: z * Phi(z) */
 } dn_activation;
 
 typedef enum { DN_QKNORM_NONE = 0, DN_QKNORM_L2 = 1, DN_QKNORM_SUM = 2 } dn_qk_norm;
@@ -405,6 +407,142 @@ typedef struct {
 } dn_block_step_args;
 
 int dn_block_step(const dn_block_step_args *args, hipStream_t stream);
+
+/* The operators around the mixer in a decoder layer. No counterpart in the
+ * reference, whose blocks end at their projections (Burn's Linear holds W as
+ * [d_input, d_output], as here). Rows are contiguous; *_stride is the number of
+ * elements between consecutive rows (at least the row's width; any alignment of
+ * the element's own). rows may be 0: the forwards then do nothing, and the
+ * backwards write zeros to the weights' gradients. Widths are at most 2^24, and
+ * every tensor is below 2^40 elements. Sums, norms and products accumulate in
+ * fp32. No output may alias an input except where said; workspaces as for the
+ * chunk calls (dn_*_workspace_bytes, 16-byte aligned, NULL: the library's). */
+
+/* sum = x + residual; out = sum / sqrt(mean(sum^2) + eps) * weight, per row of
+ * `dim` values, from the unrounded sum. With out_dtype DN_F8: scale[row] =
+ * max|out| / 448, out = the e4m3 codes of out / scale (0 where the row is all
+ * zeros), and the codes from `dim` up to the next multiple of 16 that fits in
+ * out_stride are zero, as dn_linear's 8-bit operands need them. */
+typedef struct {
+  int64_t rows, dim;
+  int64_t x_stride, residual_stride, sum_stride, out_stride;
+  double eps;
+  int32_t dtype;         /* x, residual, sum: DN_F32 or DN_BF16 */
+  int32_t weight_dtype;  /* DN_F32 or DN_BF16 */
+  int32_t out_dtype;     /* dtype, or DN_F8 */
+  const void *x;
+  const void *residual;  /* NULL: sum = x */
+  const void *weight;    /* gamma [dim] */
+  void *sum;             /* NULL: not written; may alias x or residual */
+  void *out;
+  float *scale;          /* [rows], for DN_F8 */
+} dn_add_rms_norm_args;
+
+int dn_add_rms_norm(const dn_add_rms_norm_args *args, hipStream_t stream);
+
+/* Its gradient at `sum` (as the forward wrote it): d_x (= d_residual) =
+ * inv * (d_out*weight - u * mean(d_out*weight*u)) + d_sum with u = sum * inv, and
+ * d_weight = sum over rows of d_out * u, added up in a fixed order. */
+typedef struct {
+  int64_t rows, dim;
+  int64_t sum_stride, d_out_stride, d_sum_stride, d_x_stride;
+  double eps;
+  int32_t dtype;         /* sum, d_out, d_sum, d_x */
+  int32_t weight_dtype;  /* weight, d_weight */
+  const void *sum, *weight, *d_out;
+  const void *d_sum;     /* NULL: zeros */
+  void *d_x;             /* may alias d_out or d_sum */
+  void *d_weight;        /* [dim]; NULL: not formed */
+  void *workspace;       /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_add_rms_norm_bwd_args;
+
+int dn_add_rms_norm_bwd(const dn_add_rms_norm_bwd_args *args, hipStream_t stream);
+size_t dn_add_rms_norm_bwd_workspace_bytes(const dn_add_rms_norm_bwd_args *args);
+
+/* out = act(x weight + bias) + residual, weight [in_dim, out_dim]. With dtype
+ * DN_F8: x [rows, in_dim] and weight [out_dim, in_dim] are e4m3 codes with one
+ * scale a row, the product is x_scale[row] * weight_scale[column] * (x weight^T),
+ * and both strides are multiples of 16 bytes with zero codes from in_dim up to
+ * the next multiple of 16. activation: DN_ACT_IDENTITY, SILU, RELU or GELU. */
+typedef struct {
+  int64_t rows, in_dim, out_dim;
+  int64_t x_stride, weight_stride, residual_stride, out_stride, preact_stride;
+  int32_t dtype;         /* x, weight: DN_F32, DN_BF16 or DN_F8 */
+  int32_t out_dtype;     /* out, bias, residual, preact: dtype; for DN_F8 either other */
+  int32_t activation;
+  const void *x, *weight;
+  const float *x_scale;       /* [rows], DN_F8 only */
+  const float *weight_scale;  /* [out_dim], DN_F8 only */
+  const void *bias;      /* [out_dim] or NULL */
+  const void *residual;  /* [rows, out_dim] or NULL */
+  void *out;             /* may alias residual */
+  void *preact;          /* x weight + bias, kept for the backward; or NULL */
+  void *workspace;       /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_linear_args;
+
+int dn_linear(const dn_linear_args *args, hipStream_t stream);
+size_t dn_linear_workspace_bytes(const dn_linear_args *args);
+
+/* Its gradients: d_z = d_out * act'(preact), d_x = d_z weight^T, d_weight =
+ * x^T d_z, d_bias = the sum of d_z over the rows (d_residual is d_out). Outputs
+ * that are NULL are not formed; d_weight is dense. DN_F32 or DN_BF16. */
+typedef struct {
+  int64_t rows, in_dim, out_dim;
+  int64_t x_stride, weight_stride, d_out_stride, preact_stride, d_x_stride;
+  int32_t dtype;
+  int32_t activation;
+  const void *d_out, *x, *weight;
+  const void *preact;    /* read unless the activation is the identity */
+  void *d_x, *d_weight, *d_bias;
+  void *workspace;
+  size_t workspace_bytes;
+} dn_linear_bwd_args;
+
+int dn_linear_bwd(const dn_linear_bwd_args *args, hipStream_t stream);
+size_t dn_linear_bwd_workspace_bytes(const dn_linear_bwd_args *args);
+
+/* The gated feed-forward block: h = act(x w_gate) * (x w_up),
+ * out = h w_down + residual. w_gate and w_up [dim, hidden] with one stride (so
+ * they may be the halves of one [dim, 2*hidden] matrix), w_down [hidden, dim].
+ * gate and up, if given, keep x w_gate and x w_up for the backward. h is
+ * rounded to `dtype` between the two products. */
+typedef struct {
+  int64_t rows, dim, hidden;
+  int64_t x_stride, w_in_stride, w_down_stride, residual_stride, out_stride, kept_stride;
+  int32_t dtype;
+  int32_t activation;
+  const void *x, *w_gate, *w_up, *w_down;
+  const void *residual;  /* [rows, dim] or NULL */
+  void *out;             /* may alias residual; not x */
+  void *gate, *up;       /* [rows, hidden], both or neither NULL */
+  void *workspace;
+  size_t workspace_bytes;
+} dn_gated_ffn_args;
+
+int dn_gated_ffn(const dn_gated_ffn_args *args, hipStream_t stream);
+size_t dn_gated_ffn_workspace_bytes(const dn_gated_ffn_args *args);
+
+/* Its gradients from the kept gate and up: d_h = d_out w_down^T, d_gate =
+ * d_h * up * act'(gate), d_up = d_h * act(gate), d_x = d_gate w_gate^T +
+ * d_up w_up^T, d_w_gate = x^T d_gate, d_w_up = x^T d_up, d_w_down = h^T d_out
+ * (d_residual is d_out). d_gate, d_up and h are rounded to `dtype` between the
+ * products. Outputs that are NULL are not formed (d_w_gate and d_w_up go
+ * together); the weights' gradients are dense. */
+typedef struct {
+  int64_t rows, dim, hidden;
+  int64_t x_stride, w_in_stride, w_down_stride, d_out_stride, kept_stride, d_x_stride;
+  int32_t dtype;
+  int32_t activation;
+  const void *d_out, *x, *w_gate, *w_up, *w_down, *gate, *up;
+  void *d_x, *d_w_gate, *d_w_up, *d_w_down;
+  void *workspace;
+  size_t workspace_bytes;
+} dn_gated_ffn_bwd_args;
+
+int dn_gated_ffn_bwd(const dn_gated_ffn_bwd_args *args, hipStream_t stream);
+size_t dn_gated_ffn_bwd_workspace_bytes(const dn_gated_ffn_bwd_args *args);
 
 /* How unit_lower_inverse inverts I − N (TriSolve, src/delta/tri.rs:53-64). */
 typedef enum {
