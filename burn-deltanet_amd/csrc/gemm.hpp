@@ -17,6 +17,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "activations.hpp"
 #include "dn_common.hpp"
@@ -45,8 +46,9 @@ struct GemmArgs {
   int nseg;             // contraction segments: 1 or 2
   int npair;            // products that share A: 1 or 2 (b[z] → out[z])
   int ktiles;           // k tiles of a segment
-  int split;            // workgroups along the contraction
-  int per_split;        // k tiles of each
+  int split;            // workgroups along the contraction (wide: workgroups)
+  int per_split;        // k tiles of each (wide: of the rest's share)
+  int rounds;           // wide: whole tiles of every workgroup
   int tiles_m, tiles_n;
   // epilogue
   int act;
@@ -100,22 +102,49 @@ __device__ inline Codes16 widen(const uint4& c) {
           make_uint4(two(c.z, L{}), two(c.z, H{}), two(c.w, L{}), two(c.w, H{}))};
 }
 
+// f(0), …, f(N − 1) with compile-time arguments.
+template <int... I, class F>
+__device__ inline void each_of(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ inline void each(F f) {
+  each_of(std::make_integer_sequence<int, N>{}, f);
+}
+
 // act(z) and its derivative. GELU is the exact form, z·Φ(z).
 __device__ inline float gelu_cdf(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
-__device__ inline float act_value(float z, int kind) {
-  if (kind == DN_ACT_GELU) return z * gelu_cdf(z);
-  return activate(z, kind);
-}
-__device__ inline float act_slope(float z, int kind) {
-  switch (kind) {
-    case DN_ACT_SILU: {
-      const float s = sigmoidf_(z);
-      return s * (1.0f + z * (1.0f - s));
+// a[i] = act(z[i]), and with SLOPE d[i] = act'(z[i]): one branch for eight (a
+// may be z).
+template <bool SLOPE>
+__device__ inline void act8(const float (&z)[8], int kind, float (&a)[8], float (&d)[8]) {
+  if (kind == DN_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = z[i], s = sigmoidf_(x);
+      a[i] = x * s;
+      if constexpr (SLOPE) d[i] = s * (1.0f + x * (1.0f - s));
     }
-    case DN_ACT_RELU: return z > 0.f ? 1.0f : 0.f;
-    case DN_ACT_GELU:
-      return gelu_cdf(z) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
-    default: return 1.0f;
+  } else if (kind == DN_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = z[i], c = gelu_cdf(x);
+      a[i] = x * c;
+      if constexpr (SLOPE) d[i] = c + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+    }
+  } else if (kind == DN_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = z[i];
+      a[i] = fmaxf(x, 0.f);
+      if constexpr (SLOPE) d[i] = x > 0.f ? 1.0f : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = z[i];
+      if constexpr (SLOPE) d[i] = 1.0f;
+    }
   }
 }
 
@@ -153,69 +182,121 @@ __device__ inline void store8(T* p, const float (&v)[8], int valid) {
   }
 }
 
-// The linear epilogue on eight columns of a row (z: the product, and on
-// return act's value with the residual). Shared by the tile kernel, the
-// few-rows kernel and the join of split contractions.
-template <class TO>
-__device__ inline void linear_tail(const GemmArgs& p, int z, int64_t row, int col, float (&v)[8]) {
+// Eight adjacent values as they lie in memory, until they are used.
+template <class T>
+struct Raw8 {
+  static constexpr int kWords = 2 * int(sizeof(T));
+  uint32_t w[kWords];
+  __device__ inline void load(const T* p, int valid) {
+    if (valid >= 8) {
+      __builtin_memcpy(w, p, sizeof(w));
+    } else {
+      float v[8];
+      load8(p, v, valid);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pk_bf16(v[2 * i], v[2 * i + 1]);
+      }
+    }
+  }
+  __device__ inline void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+      unpack8(make_uint4(w[0], w[1], w[2], w[3]), v);
+    }
+  }
+};
+
+// The epilogues on eight columns of a row, each in two parts, so that a caller
+// can have several rows' loads in flight: what it reads (Tail), then the rest.
+// Shared by the tile kernels, the few-rows kernel and the join of split
+// contractions.
+template <class TO, int EPI>
+struct Tail {
+  Raw8<TO> x, y;  // linear: the residual; d_gated: the kept gate and up
+};
+template <class TO, int EPI>
+__device__ inline void tail_load(const GemmArgs& p, int64_t row, int col, Tail<TO, EPI>& t) {
   const int valid = p.N - col;
-  if (p.row_scale) {
-    const float rs = p.row_scale[row];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < valid) v[i] *= rs * p.col_scale[col + i];
+  if constexpr (EPI == kEpiLinear) {
+    if (p.residual) t.x.load(static_cast<const TO*>(p.residual) + row * p.ldr + col, valid);
+  } else if constexpr (EPI == kEpiDGated) {
+    t.x.load(static_cast<const TO*>(p.preact) + row * p.ldp + col, valid);
+    t.y.load(static_cast<const TO*>(p.up) + row * p.ldp + col, valid);
   }
-  if (p.bias) {
-    float b[8];
-    load8(static_cast<const TO*>(p.bias) + col, b, valid);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += b[i];
-  }
-  if (p.preact) store8(static_cast<TO*>(p.preact) + row * p.ldp + col, v, valid);
-  if (p.act != DN_ACT_IDENTITY) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], p.act);
-  }
-  if (p.residual) {
-    float r[8];
-    load8(static_cast<const TO*>(p.residual) + row * p.ldr + col, r, valid);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
-  }
-  store8(static_cast<TO*>(z ? p.out[1] : p.out[0]) + row * p.ldo + col, v, valid);
 }
-// h = act(g)·u, and the kept g and u.
-template <class TO>
-__device__ inline void gated_tail(const GemmArgs& p, int64_t row, int col, const float (&g)[8],
-                                  const float (&u)[8]) {
+// v: the product (gated: gate's, and u up's). z: which of a pair of products.
+template <class TO, int EPI>
+__device__ inline void tail_store(const GemmArgs& p, int z, int64_t row, int col, float (&v)[8],
+                                  const float (&u)[8], Tail<TO, EPI>& t) {
   const int valid = p.N - col;
-  if (p.preact) {
-    store8(static_cast<TO*>(p.preact) + row * p.ldp + col, g, valid);
-    store8(static_cast<TO*>(p.up) + row * p.ldp + col, u, valid);
-  }
-  float h[8];
+  float none[8];
+  if constexpr (EPI == kEpiLinear) {
+    if (p.row_scale) {
+      const float rs = p.row_scale[row];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = act_value(g[i], p.act) * u[i];
-  store8(static_cast<TO*>(p.out[0]) + row * p.ldo + col, h, valid);
+      for (int i = 0; i < 8; ++i)
+        if (i < valid) v[i] *= rs * p.col_scale[col + i];
+    }
+    if (p.bias) {
+      float b[8];
+      load8(static_cast<const TO*>(p.bias) + col, b, valid);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    if (p.preact) store8(static_cast<TO*>(p.preact) + row * p.ldp + col, v, valid);
+    if (p.act != DN_ACT_IDENTITY) act8<false>(v, p.act, v, none);
+    if (p.residual) {
+      float r[8];
+      t.x.get(r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    store8(static_cast<TO*>(z ? p.out[1] : p.out[0]) + row * p.ldo + col, v, valid);
+  } else if constexpr (EPI == kEpiGated) {
+    // h = act(g)·u, and the kept g and u.
+    if (p.preact) {
+      store8(static_cast<TO*>(p.preact) + row * p.ldp + col, v, valid);
+      store8(static_cast<TO*>(p.up) + row * p.ldp + col, u, valid);
+    }
+    act8<false>(v, p.act, v, none);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= u[i];
+    store8(static_cast<TO*>(p.out[0]) + row * p.ldo + col, v, valid);
+  } else {
+    // From d_h (v) and the kept g and u: d_g = d_h·u·act'(g), d_u = d_h·act(g),
+    // and h again for the down projection's weight gradient.
+    float dg[8], h[8], kept[8];
+    t.x.get(kept);
+    act8<true>(kept, p.act, h, dg);
+    t.y.get(kept);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dg[i] *= v[i] * kept[i];
+      v[i] *= h[i];
+      h[i] *= kept[i];
+    }
+    store8(static_cast<TO*>(p.out[0]) + row * p.ldo + col, dg, valid);
+    store8(static_cast<TO*>(p.out[1]) + row * p.ldo + col, v, valid);
+    store8(static_cast<TO*>(p.h) + row * p.ldo + col, h, valid);
+  }
 }
-// From d_h and the kept g and u: d_g = d_h·u·act'(g), d_u = d_h·act(g), and h
-// again for the down projection's weight gradient.
-template <class TO>
-__device__ inline void dgated_tail(const GemmArgs& p, int64_t row, int col, const float (&dh)[8]) {
-  const int valid = p.N - col;
-  float g[8], u[8], dg[8], du[8], h[8];
-  load8(static_cast<const TO*>(p.preact) + row * p.ldp + col, g, valid);
-  load8(static_cast<const TO*>(p.up) + row * p.ldp + col, u, valid);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = act_value(g[i], p.act);
-    dg[i] = dh[i] * u[i] * act_slope(g[i], p.act);
-    du[i] = dh[i] * a;
-    h[i] = a * u[i];
+// Both parts, or the sums of a split product to the workspace.
+template <class TO, int EPI>
+__device__ inline void finish8(const GemmArgs& p, int z, int sp, int64_t row, int col,
+                               float (&v)[8], const float (&u)[8], Tail<TO, EPI>& t) {
+  if (p.partial) {
+    float* to = p.partial + (int64_t(sp * p.npair + z) * p.M + row) * p.ldpart + col;
+    store8(to, v, p.N - col);
+    if constexpr (EPI == kEpiGated) store8(to + p.N, u, p.N - col);
+  } else {
+    tail_store<TO, EPI>(p, z, row, col, v, u, t);
   }
-  store8(static_cast<TO*>(p.out[0]) + row * p.ldo + col, dg, valid);
-  store8(static_cast<TO*>(p.out[1]) + row * p.ldo + col, du, valid);
-  store8(static_cast<TO*>(p.h) + row * p.ldo + col, h, valid);
 }
 
 // One HBM → LDS copy of 16 bytes a lane: lane i's word goes to `lds` + 16·i.
@@ -227,6 +308,24 @@ __device__ inline void copy_to_lds(const char* src, uint32_t lds) {
                : "s"(lds), "v"(src)
                : "memory");
 }
+// c += b·a with c held in accumulation registers. The wide kernel's 256 sums
+// fill that half of the register file; left to itself the compiler moves them
+// between the halves at every branch (276 moves a k tile of 128 products, and
+// spills). It does not see a matrix instruction here: settle_acc() is owed
+// before anything else reads the sums.
+__device__ inline void mfma16_acc(const uint4& b, const uint4& a, f32x4& c) {
+  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+      : "+a"(c)
+      : "v"(__builtin_bit_cast(bf16x8, b)), "v"(__builtin_bit_cast(bf16x8, a)));
+}
+// The wait that a matrix instruction's result needs before another kind of
+// instruction reads it, tied to eight of the sums.
+__device__ inline void settle_acc(f32x4 (&c)[8]) {
+  asm volatile("s_nop 15\n\ts_nop 15"
+               : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]),
+                 "+a"(c[6]), "+a"(c[7]));
+}
+
 template <int N>
 __device__ inline void wait_copies() {  // at most N of this wave's copies outstanding
   static_assert(N < 64, "vmcnt");
@@ -559,36 +658,407 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     constexpr int kPer = EPI == kEpiGated ? 4 : 8;  // lanes to a row
+    constexpr int kIts = 32 * kPer / 64;
+    Tail<TO, EPI> tails[kIts];
+    const int col = col0 + (lane % kPer) * 8, c = (lane % kPer) * 8;
+    auto row_of = [&](int it) {
+      return int64_t(row0) + half * 32 + it * (64 / kPer) + lane / kPer;
+    };
 #pragma unroll
-    for (int it = 0; it < 32 * kPer / 64; ++it) {
-      const int r = it * (64 / kPer) + lane / kPer, c = (lane % kPer) * 8;
-      const int64_t row = row0 + half * 32 + r;
-      const int col = col0 + c;
+    for (int it = 0; it < kIts; ++it)
+      if (!p.partial && row_of(it) < p.M && col < p.N)
+        tail_load<TO, EPI>(p, row_of(it), col, tails[it]);
+#pragma unroll
+    for (int it = 0; it < kIts; ++it) {
+      const float* at = stage + (it * (64 / kPer) + lane / kPer) * kLd + c;
       float v[8], u[8];
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stage + r * kLd + c);
-      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stage + r * kLd + c + 4);
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(at);
+      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(at + 4);
       if constexpr (EPI == kEpiGated) {
-        *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stage + r * kLd + 32 + c);
-        *reinterpret_cast<float4*>(u + 4) =
-            *reinterpret_cast<const float4*>(stage + r * kLd + 36 + c);
+        *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(at + 32);
+        *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(at + 36);
       }
-      if (row < p.M && col < p.N) {
-        if (p.partial) {
-          float* at = p.partial + (int64_t(sp * p.npair + z) * p.M + row) * p.ldpart + col;
-          store8(at, v, p.N - col);
-          if constexpr (EPI == kEpiGated)
-            store8(at + p.N, u, p.N - col);
-        } else if constexpr (EPI == kEpiLinear) {
-          linear_tail<TO>(p, z, row, col, v);
-        } else if constexpr (EPI == kEpiGated) {
-          gated_tail<TO>(p, row, col, v, u);
-        } else {
-          dgated_tail<TO>(p, row, col, v);
+      if (row_of(it) < p.M && col < p.N)
+        finish8<TO, EPI>(p, z, sp, row_of(it), col, v, u, tails[it]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The same product for large sizes: 256 × 256 tiles, four waves of 128 × 128,
+// one to a SIMD, so that a fragment read from LDS feeds eight products (eight
+// waves of 128 × 64 read 1.5 times as many bytes).
+//
+// LDS holds two k tiles (128 bytes of every row) of B and three of A: all of a
+// CU's 160 KB. A tile is 16 slots: for each half of its k, each of the wave's
+// eight row blocks against all eight column blocks. The order is fixed in the
+// source (sched_barrier): a wave issues in order, so a memory instruction
+// stands between any two or three products and issues while they run. In slots
+// 0…5 the fragments of the tile's second half are read; at slot 8, where the
+// wave holds all it needs of the tile, is the tile's one barrier; in slots
+// 8…13 the fragments of the next tile's first half are read. Copies go out one
+// a slot, A's of tile t + 2 in slots 0…7, B's in 8…15: the four waves' then
+// take half of the vector memory path's time; two a slot take all of it, and
+// the waves wait for it in place of the matrix unit.
+//
+// Copies take their address as a scalar base and a 32-bit offset: with 64-bit
+// addresses in registers 16 loads beside 128 products take 1200 ns, like this
+// 1116, without any loads 1096.
+//
+// "col" operands lie in LDS as subtiles of 128 columns, so that every copy
+// instruction reads one matrix; gated: gate's and up's.
+//
+// One workgroup to a CU. Where the tiles are no whole number of rounds, the
+// rest's k tiles are dealt out evenly (per_split to a workgroup): parts of a
+// tile leave their sums in the workspace, and wide_join_kernel adds them in
+// the order of k.
+template <class T, class TO, bool ACOL, bool BCOL, int EPI>
+__global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
+  using namespace gemm;
+  using E = Elem<T>;
+  constexpr int CH = E::kCh, KT = E::kKT, ES = int(sizeof(T));
+  constexpr int kHalf = 256 * 128;  // bytes of an operand's tile
+  constexpr int NW = 8;             // copies of an operand's tile a thread
+  __shared__ __attribute__((aligned(16))) char smem[5 * kHalf];  // A, A, A, B, B
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int s = lane & 15, q = lane >> 4;
+
+  // The workgroup's work: whole tiles while there are rounds of them for all
+  // workgroups, then its share of the rest's k tiles. Workgroups go round the
+  // eight XCDs: by `place` each XCD has a contiguous range of tiles, ordered in
+  // bands of 8 tile rows, so its 32 CUs share operand tiles in its L2.
+  const int groups = gridDim.x, tiles = p.tiles_m * p.tiles_n, nk = p.ktiles * p.nseg;
+  const int xcd = blockIdx.x & 7, per_xcd = groups >> 3, more_xcd = groups & 7;
+  const int place = xcd * per_xcd + min(xcd, more_xcd) + (blockIdx.x >> 3);
+  int round = 0;
+  int64_t unit = int64_t(place) * p.per_split;  // of the rest: tile · nk + k tile
+  const int64_t unit_end =
+      min(unit + p.per_split, int64_t(tiles * p.npair - p.rounds * groups) * nk);
+  while (true) {
+  int id, t0, t1, slot_no = -1;  // slot_no: where a part of a tile leaves its sums
+  if (round < p.rounds) {
+    id = round * groups + place;
+    t0 = 0;
+    t1 = nk;
+    ++round;
+  } else {
+    if (unit >= unit_end) break;
+    const int rest = int(unit / nk);
+    t0 = int(unit - int64_t(rest) * nk);
+    t1 = int(min(int64_t(nk), t0 + (unit_end - unit)));
+    unit += t1 - t0;
+    id = p.rounds * groups + rest;
+    if (t1 - t0 < nk) slot_no = place + rest;
+  }
+  const int z = id / tiles;
+  int tm, tn;
+  {
+    const int t = id - z * tiles, band = 8 * p.tiles_n, g = t / band, first = g * 8;
+    const int rows = min(8, p.tiles_m - first), r = t - g * band;
+    tm = first + r % rows;
+    tn = r / rows;
+  }
+  constexpr int kCols = EPI == kEpiGated ? 128 : 256;
+  const int m0 = tm * 256, n0 = tn * kCols;
+
+  // Word w of a thread's copies of an operand's tile: (r, c) is its row and
+  // 16-byte word ("row"), or its k and word of the subtile `sub` ("col").
+  auto word = [&](auto col, int w, int& r, int& c, int& sub) {
+    const int L = (w * 4 + wave) * 64 + lane;
+    if constexpr (decltype(col)::value) {
+      sub = (w * 4) >> 4;  // 16 KB subtiles: 1024 words, four of each thread
+      const int l = L & 1023;
+      r = l >> (CH == 8 ? 4 : 5);
+      c = (l & (128 / CH - 1)) ^ swizzle_col<T>(r);
+    } else {
+      sub = 0;
+      r = L >> 3;
+      c = (L & 7) ^ swizzle_row(r);
+    }
+  };
+  static_assert(!(ACOL || BCOL) || sizeof(T) == 2, "subtiles of 1024 words");
+  using AC = std::integral_constant<bool, ACOL>;
+  using BC = std::integral_constant<bool, BCOL>;
+
+  // Byte offsets of the copies' sources from the tile's base: rows past the end
+  // moved back to the last one, words to the last whole one (what they give is
+  // not stored).
+  uint32_t oa[NW], ob[NW];
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    int r, c, sub;
+    word(AC{}, w, r, c, sub);
+    if constexpr (ACOL)
+      oa[w] = uint32_t(r * p.lda) + uint32_t(min(sub * 128 + c * CH, p.M - CH - m0) * ES);
+    else
+      oa[w] = uint32_t(min(r, p.M - 1 - m0) * p.lda) + uint32_t(c * 16);
+    word(BC{}, w, r, c, sub);
+    if constexpr (BCOL)
+      ob[w] = uint32_t(r * p.ldb) +
+              uint32_t(min((EPI == kEpiGated ? 0 : sub * 128) + c * CH, p.N - CH - n0) * ES);
+    else
+      ob[w] = uint32_t(min(r, p.N - 1 - n0) * p.ldb) + uint32_t(c * 16);
+  }
+  // The tile being copied: its bases, and its place in its segment, followed
+  // step by step (a division and a load of the segment's pointers a tile would
+  // hold up the wave). `plain`: it is inside this workgroup's range, and not a
+  // segment's ragged last one.
+  const int segment0 = t0 / p.ktiles;
+  int kt = t0 - segment0 * p.ktiles, left = t1 - t0;
+  const char* pa = segment0 ? p.a[1] : p.a[0];
+  const char* pb = segment0 || (p.npair == 2 && z) ? p.b[1] : p.b[0];
+  const int64_t skip_a = ACOL ? int64_t(m0) * ES : int64_t(m0) * p.lda;
+  const int64_t skip_b = BCOL ? int64_t(n0) * ES : int64_t(n0) * p.ldb;
+  const int64_t step_a = ACOL ? p.lda * KT : 128, step_b = BCOL ? p.ldb * KT : 128;
+  const char* ba = pa + skip_a + kt * step_a;
+  const char* bb = pb + skip_b + kt * step_b;
+  const char* bu = p.b[1] + skip_b + kt * step_b;  // gated: up
+  const char *second_a = p.a[1] + skip_a, *second_b = p.b[1] + skip_b;
+  const int whole_tiles = p.K / KT, ktiles = p.ktiles;
+  auto plain = [&] { return left > 0 && kt < whole_tiles; };
+  auto advance = [&] {
+    --left;
+    ++kt;
+    ba += step_a;
+    bb += step_b;
+    bu += step_b;
+    if (kt == ktiles) {
+      kt = 0;
+      ba = second_a;
+      bb = second_b;
+      pa = p.a[1];
+      pb = p.b[1];
+    }
+  };
+  const uint32_t lds0 = lds_address(smem) + uint32_t(wave) * 1024;
+  auto copy = [&](uint32_t at, uint32_t offset, const char* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds0 + at), "v"(offset), "s"(base)
+                 : "memory");
+  };
+  // Buffers: A's of tile t is (t − t0) % 3, B's (t − t0) % 2.
+  auto copy_a = [&](int buf, int w) { copy(uint32_t(buf * kHalf + w * 4096), oa[w], ba); };
+  auto copy_b = [&](int buf, int w) {
+    copy(uint32_t((3 + buf) * kHalf + w * 4096), ob[w],
+         EPI == kEpiGated && w >= NW / 2 ? bu : bb);
+  };
+  auto masked = [&](const char* base, int64_t ldx, bool col, int k, int i, int extent) {
+    const int major = col ? k : i, minor = col ? i : k;
+    const int major_end = col ? p.K : extent, minor_end = col ? extent : p.K;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (major < major_end && minor < minor_end)  // whole words: the widths are
+      v = *reinterpret_cast<const uint4*>(base + int64_t(major) * ldx + int64_t(minor) * ES);
+    return v;
+  };
+  // A segment's ragged last tile, through registers with masks.
+  auto ragged_a = [&](int buf) {
+    const int k0 = kt * KT;
+#pragma unroll 1
+    for (int w = 0; w < NW; ++w) {
+      int r, c, sub;
+      word(AC{}, w, r, c, sub);
+      *reinterpret_cast<uint4*>(smem + buf * kHalf + (w * 4 + wave) * 1024 + lane * 16) =
+          ACOL ? masked(pa, p.lda, true, k0 + r, m0 + sub * 128 + c * CH, p.M)
+               : masked(pa, p.lda, false, k0 + c * CH, m0 + r, p.M);
+    }
+  };
+  auto ragged_b = [&](int buf) {
+    const int k0 = kt * KT;
+#pragma unroll 1
+    for (int w = 0; w < NW; ++w) {
+      int r, c, sub;
+      word(BC{}, w, r, c, sub);
+      *reinterpret_cast<uint4*>(smem + (3 + buf) * kHalf + (w * 4 + wave) * 1024 + lane * 16) =
+          BCOL ? masked(EPI == kEpiGated && sub ? p.b[1] : pb, p.ldb, true, k0 + r,
+                        n0 + (EPI == kEpiGated ? 0 : sub * 128) + c * CH, p.N)
+               : masked(pb, p.ldb, false, k0 + c * CH, n0 + r, p.N);
+    }
+  };
+
+  // Fragment of 16-row block `blk` of 128-row subtile `sub`, half kk.
+  auto frag = [&](const char* tile, auto col, int sub, int blk, int kk) -> uint4 {
+    if constexpr (decltype(col)::value) {
+      const int g = (s >> 2) | ((q & 1) << 2);
+      const char* at = tile + sub * 16384 + (32 * kk + 8 * q + (s >> 2)) * 256 + ((blk ^ g) * 32) +
+                       (s & 3) * 8;
+      typedef __attribute__((address_space(3))) i16x4* P;
+      const uint2 l = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at));
+      const uint2 h =
+          __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 1024)));
+      return make_uint4(l.x, l.y, h.x, h.y);
+    } else {
+      return *reinterpret_cast<const uint4*>(tile + (sub * 128 + blk * 16 + s) * 128 +
+                                             (((4 * kk + q) ^ swizzle_row(s)) << 4));
+    }
+  };
+
+  f32x4 acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint4 fa[2][8], fb[2][8];  // [half][block]
+  constexpr bool kF8 = sizeof(T) == 1;
+  Codes16 wb[kF8 ? 8 : 1];
+  // Fragment n of half kk's sixteen, in the order of their first use.
+  auto read = [&](const char* a, const char* b, auto kk_no, auto n_no) {
+    constexpr int kk = decltype(kk_no)::value, n = decltype(n_no)::value;
+    if constexpr (n < 8)
+      fb[kk][n] = EPI == kEpiGated ? frag(b, BC{}, n >> 2, wn * 4 + (n & 3), kk)
+                                   : frag(b, BC{}, wn, n, kk);
+    else
+      fa[kk][n - 8] = frag(a, AC{}, wm, n - 8, kk);
+  };
+
+  {
+    // Tiles t0 and t0 + 1.
+    for (int d = 0; d < 2; ++d) {
+      if (plain()) {
+        each<NW>([&](auto w) {
+          copy_a(d, w);
+          copy_b(d, w);
+        });
+      } else if (left > 0) {
+        ragged_a(d);
+        ragged_b(d);
+      }
+      advance();
+    }
+    wait_copies<0>();
+    __syncthreads();
+    const char *sa = smem, *sb = smem + 3 * kHalf;
+    using Half0 = std::integral_constant<int, 0>;
+    using Half1 = std::integral_constant<int, 1>;
+    each<16>([&](auto n) { read(sa, sb, Half0{}, n); });
+    int abuf = 0;
+    for (int t = t0; t < t1; ++t) {
+      const int bbuf = (t - t0) & 1, anext = abuf == 2 ? 0 : abuf + 1;
+      const int afill = anext == 2 ? 0 : anext + 1;  // of t − 1 and t + 2
+      const char *ca = smem + abuf * kHalf, *cb = smem + (3 + bbuf) * kHalf;
+      const char *na = smem + anext * kHalf, *nb = smem + (3 + (bbuf ^ 1)) * kHalf;
+      const bool more = plain();  // tile t + 2
+      if (!more && left > 0) ragged_a(afill);
+      auto work = [&](auto slot_no) {
+        constexpr int slot = decltype(slot_no)::value, kk = slot >> 3, i = slot & 7;
+        Codes16 a;
+        if constexpr (kF8) {
+          if constexpr (i == 0)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wb[j] = widen(fb[kk][j]);
+          a = widen(fa[kk][i]);
+        }
+        each<8>([&](auto jn) {
+          constexpr int j = decltype(jn)::value;
+          if constexpr (kF8) {
+            mfma16_acc(wb[j].lo, a.lo, acc[i][j]);
+            mfma16_acc(wb[j].hi, a.hi, acc[i][j]);
+          } else {
+            mfma16_acc(fb[kk][j], fa[kk][i], acc[i][j]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          // Sixteen fragments, three a slot: of this tile's second half from slot
+          // 0 on, of the next tile's first half from slot 8 on (after the last
+          // tile they are of no use).
+          constexpr int n = 3 * i + (j >> 1);
+          if constexpr ((j == 1 || j == 3 || j == 5) && n < 16) {
+            if constexpr (slot < 8) read(ca, cb, Half1{}, std::integral_constant<int, n>{});
+            else read(na, nb, Half0{}, std::integral_constant<int, n>{});
+          }
+          if constexpr (j == 6) {
+            if constexpr (slot < 8) {
+              if (more) copy_a(afill, i);
+            } else {
+              if (more) copy_b(bbuf, i);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      };
+      each<8>(work);
+      // A's and B's tile t + 1 have landed once no more copies are out than
+      // those of A's t + 2.
+      if (more) wait_copies<NW>();
+      else wait_copies<0>();
+      lds_barrier();
+      if (!more && left > 0) ragged_b(bbuf);
+      each<8>([&](auto n) { work(std::integral_constant<int, 8 + n.value>{}); });
+      advance();
+      abuf = anext;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) settle_acc(acc[i]);
+
+  // Epilogue: half of the wave's rows (64 by 128 columns) at a time through its
+  // own LDS, 16-byte words XORed by row over the banks.
+  float4* stage = reinterpret_cast<float4*>(smem) + wave * 64 * 32;
+  auto at = [&](int r, int c) -> float4& { return stage[r * 32 + (c ^ (r & 15))]; };
+  auto flush = [&](auto half) {
+    constexpr int kHalfRows = decltype(half)::value;
+    constexpr int kPer = EPI == kEpiGated ? 8 : 16;  // lanes to a row
+    constexpr int kAtOnce = EPI == kEpiGated ? 4 : 8;
+    const int64_t row0 = m0 + wm * 128 + kHalfRows * 64;
+    const int col = n0 + wn * (EPI == kEpiGated ? 64 : 128) + (lane % kPer) * 8;
+    Tail<TO, EPI> tails[kAtOnce];
+    auto fetch = [&](int it) {
+#pragma unroll
+      for (int n = 0; n < kAtOnce; ++n) {
+        const int64_t row = row0 + (it + n) * (64 / kPer) + lane / kPer;
+        if (slot_no < 0 && row < p.M && col < p.N) tail_load<TO, EPI>(p, row, col, tails[n]);
+      }
+    };
+    fetch(0);
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const f32x4 v = acc[kHalfRows * 4 + ii][j];
+        at(ii * 16 + s, 4 * j + q) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // What the epilogue reads for eight rows is in flight at a time, the first
+    // eight's since before the sums went to LDS.
+#pragma unroll 1
+    for (int it = 0; it < kPer; it += kAtOnce) {
+      auto local = [&](int n) { return (it + n) * (64 / kPer) + lane / kPer; };
+      if (it > 0) fetch(it);
+      float v[kAtOnce][8], u[EPI == kEpiGated ? kAtOnce : 1][8];
+#pragma unroll
+      for (int n = 0; n < kAtOnce; ++n) {
+        const int r = local(n), c = 2 * (lane % kPer);
+        *reinterpret_cast<float4*>(v[n]) = at(r, c);
+        *reinterpret_cast<float4*>(v[n] + 4) = at(r, c + 1);
+        if constexpr (EPI == kEpiGated) {
+          *reinterpret_cast<float4*>(u[n]) = at(r, 16 + c);
+          *reinterpret_cast<float4*>(u[n] + 4) = at(r, 16 + c + 1);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kAtOnce; ++n) {
+        if (slot_no >= 0) {  // a part: its sums to the workspace, gate's then up's
+          float* to = p.partial +
+                      ((int64_t(slot_no) * 256 + int(row0 - m0) + local(n)) << 8) + (col - n0);
+          store8(to, v[n], 8);
+          if constexpr (EPI == kEpiGated) store8(to + 128, u[n], 8);
+        } else if (row0 + local(n) < p.M && col < p.N) {
+          tail_store<TO, EPI>(p, z, row0 + local(n), col, v[n], u[EPI == kEpiGated ? n : 0],
+                              tails[n]);
         }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  flush(std::integral_constant<int, 0>{});
+  flush(std::integral_constant<int, 1>{});
+  __syncthreads();
   }
 }
 

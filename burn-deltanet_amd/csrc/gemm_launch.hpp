@@ -19,8 +19,13 @@ hipError_t gemm_go(const GemmArgs& g, hipStream_t stream) {
 
 template <class T, class TO, bool ACOL, bool BCOL, int EPI, bool STAGED>
 hipError_t gemm_tile(const GemmArgs& g, GemmTile tile, hipStream_t stream) {
-  if (tile == kTile256)
-    return gemm_go<T, TO, ACOL, BCOL, 256, 256, 2, 4, EPI, STAGED>(g, stream);
+  if constexpr (!STAGED && sizeof(T) < 4) {
+    if (tile == kTileWide) {
+      hipLaunchKernelGGL((gemm_wide_kernel<T, TO, ACOL, BCOL, EPI>), dim3(unsigned(g.split)),
+                         dim3(256), 0, stream, g);
+      return hipGetLastError();
+    }
+  }
   return gemm_go<T, TO, ACOL, BCOL, 128, 128, 2, 2, EPI, STAGED>(g, stream);
 }
 

@@ -35,6 +35,8 @@ __global__ __launch_bounds__(kJoinThreads) void gemm_join_kernel(GemmArgs p) {
   const int valid = p.N - col;
   const int64_t hop = int64_t(p.npair) * p.M * p.ldpart;
   const float* at = p.partial + (int64_t(z) * p.M + row) * p.ldpart + col;
+  gemm::Tail<TO, EPI> tail;
+  gemm::tail_load<TO, EPI>(p, row, col, tail);
   float v[8] = {}, u[8] = {};
   for (int sp = 0; sp < p.split; ++sp, at += hop) {
     float w[8];
@@ -47,9 +49,48 @@ __global__ __launch_bounds__(kJoinThreads) void gemm_join_kernel(GemmArgs p) {
       for (int e = 0; e < 8; ++e) u[e] += w[e];
     }
   }
-  if constexpr (EPI == kEpiLinear) gemm::linear_tail<TO>(p, z, row, col, v);
-  else if constexpr (EPI == kEpiGated) gemm::gated_tail<TO>(p, row, col, v, u);
-  else gemm::dgated_tail<TO>(p, row, col, v);
+  gemm::tail_store<TO, EPI>(p, z, row, col, v, u, tail);
+}
+
+// The same for the wide kernel's split tiles: workgroup w has the rest's k
+// tiles w·per … (w + 1)·per − 1, and its part of the rest's tile t is slot
+// w + t of the workspace. A workgroup of this kernel takes 8 rows of a tile.
+template <class TO, int EPI>
+__global__ __launch_bounds__(kJoinThreads) void wide_join_kernel(GemmArgs p) {
+  constexpr int kPer = EPI == kEpiGated ? 16 : 32;  // threads to a row
+  constexpr int kRows = kJoinThreads / kPer;
+  const int t = blockIdx.x, nk = p.ktiles * p.nseg, tiles = p.tiles_m * p.tiles_n;
+  const int64_t u0 = int64_t(t) * nk;
+  const int w0 = int(u0 / p.per_split), w1 = int((u0 + nk - 1) / p.per_split);
+  if (w0 == w1) return;  // in one piece
+  const int id = p.rounds * p.split + t, z = id / tiles;
+  int tm, tn;
+  {
+    const int i = id - z * tiles, band = 8 * p.tiles_n, g = i / band, first = g * 8;
+    const int rows = min(8, p.tiles_m - first), r = i - g * band;
+    tm = first + r % rows;
+    tn = r / rows;
+  }
+  const int r = blockIdx.y * kRows + threadIdx.x / kPer, c = (threadIdx.x % kPer) * 8;
+  const int64_t row = int64_t(tm) * 256 + r;
+  const int col = tn * (EPI == kEpiGated ? 128 : 256) + c;
+  if (row >= p.M || col >= p.N) return;
+  gemm::Tail<TO, EPI> tail;
+  gemm::tail_load<TO, EPI>(p, row, col, tail);
+  float v[8] = {}, u[8] = {};
+  for (int w = w0; w <= w1; ++w) {
+    const float* at = p.partial + ((int64_t(w + t) * 256 + r) << 8) + c;
+    float x[8];
+    gemm::load8(at, x, 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x[e];
+    if constexpr (EPI == kEpiGated) {
+      gemm::load8(at + 128, x, 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] += x[e];
+    }
+  }
+  gemm::tail_store<TO, EPI>(p, z, row, col, v, u, tail);
 }
 
 // d_z = d_out·act'(z) and the column sums of d_z, over a strip of rows: a
@@ -77,8 +118,10 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
       if (p.z) {
         float z[8];
         gemm::load8(static_cast<const T*>(p.z) + r * p.ldz + col, z, valid);
+        float slope[8];
+        gemm::act8<true>(z, p.act, z, slope);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= gemm::act_slope(z[i], p.act);
+        for (int i = 0; i < 8; ++i) d[i] *= slope[i];
       }
       if (p.dz) gemm::store8(static_cast<T*>(p.dz) + r * p.lddz + col, d, valid);
 #pragma unroll
@@ -115,61 +158,13 @@ bool at16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 // How one product is cut into workgroups.
 struct Plan {
   GemmTile tile;
-  int tiles_m, tiles_n, ktiles, split, per_split;
+  bool copyable;
+  int tiles_m, tiles_n, ktiles, split, per_split, rounds;
   size_t partial_bytes;
 };
 
-Plan plan_product(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, bool gated) {
-  const int kt = int(128 / elem_size(dtype));
-  Plan best{};
-  double best_cost = 0;
-  for (int big = 0; big < 2; ++big) {
-    Plan p{};
-    const int b = big ? 256 : 128;
-    p.tile = big ? kTile256 : kTile128;
-    p.tiles_m = int(ceil_div(M, b));
-    p.tiles_n = int(ceil_div(N, gated ? b / 2 : b));
-    p.ktiles = int(ceil_div(K, kt));
-    const int64_t ksteps = std::max<int64_t>(1, int64_t(p.ktiles) * nseg);
-    const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair;
-    const int slots = device_cu_count() * (big ? 1 : 2);
-    const double unit = big ? 1.0 : 0.56;  // a k tile's time on a full machine
-    const int most = int(std::min<int64_t>(std::max<int64_t>(1, ksteps / 4), 64));
-    for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
-      const int64_t per = ceil_div(ksteps, s);
-      const int split = int(ceil_div(ksteps, per));
-      if (tiles * split > (int64_t(1) << 30)) break;
-      const double rounds = double(ceil_div(tiles * split, slots));
-      double cost = rounds * (double(per) + 6.0) * unit;
-      if (split > 1)  // partial sums out and in, at a CU's share of the memory's rate
-        cost += 8.0 + double(M) * N * (gated ? 2 : 1) * npair * split * 8.0 / 4.0e6;
-      if (best.split == 0 || cost < best_cost) {
-        best_cost = cost;
-        p.split = split;
-        p.per_split = int(per);
-        best = p;
-      }
-      if (s > 1 && tiles * s >= 4 * int64_t(slots)) break;
-    }
-  }
-  if (best.split > 1)
-    best.partial_bytes = align_up(size_t(best.split) * npair * size_t(M) *
-                                      size_t(gated ? 2 * N : align_up(size_t(N), 4)) * 4, 256);
-  return best;
-}
-
-void apply(GemmArgs& g, const Plan& p, bool gated, float* partial) {
-  g.tiles_m = p.tiles_m;
-  g.tiles_n = p.tiles_n;
-  g.ktiles = p.ktiles;
-  g.split = p.split;
-  g.per_split = p.per_split;
-  g.partial = p.split > 1 ? partial : nullptr;
-  g.ldpart = gated ? 2 * int64_t(g.N) : int64_t(align_up(size_t(g.N), 4));
-}
-
 // Whether every operand row lies at 16-byte steps and holds whole words.
-bool copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
+bool is_copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
   const int64_t ch = int64_t(16 / elem_size(dtype));
   const bool acol = form == kFormTN, bcol = form != kFormNT;
   bool ok = at16(g.a[0]) && at16(g.b[0]) && g.lda % 16 == 0 && g.ldb % 16 == 0;
@@ -180,35 +175,136 @@ bool copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
   return ok;
 }
 
-template <class TO>
-hipError_t join_typed(const GemmArgs& g, GemmEpi epi, hipStream_t stream) {
-  const int64_t n = int64_t(g.M) * ((g.N + 7) / 8) * g.npair;
-  const dim3 grid(unsigned(ceil_div(n, kJoinThreads)));
-  if (epi == kEpiLinear)
-    hipLaunchKernelGGL((gemm_join_kernel<TO, kEpiLinear>), grid, dim3(kJoinThreads), 0, stream, g);
-  else if (epi == kEpiGated)
-    hipLaunchKernelGGL((gemm_join_kernel<TO, kEpiGated>), grid, dim3(kJoinThreads), 0, stream, g);
-  else
-    hipLaunchKernelGGL((gemm_join_kernel<TO, kEpiDGated>), grid, dim3(kJoinThreads), 0, stream, g);
+// The wide kernel: one workgroup a CU, whole tiles in rounds, the rest's k
+// tiles dealt out. In k tiles' time: a tile's start and end cost about 8.
+Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, bool gated,
+               double* cost) {
+  Plan p{};
+  p.tile = kTileWide;
+  p.tiles_m = int(ceil_div(M, 256));
+  p.tiles_n = int(ceil_div(N, gated ? 128 : 256));
+  p.ktiles = int(ceil_div(K, int64_t(128 / elem_size(dtype))));
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair, nk = int64_t(p.ktiles) * nseg;
+  const int64_t cus = device_cu_count();
+  constexpr double kEnds = 8.0;
+  p.rounds = int(tiles / cus);
+  const int64_t rest = tiles - p.rounds * cus;
+  double c = p.rounds * (double(nk) + kEnds);
+  p.split = int(p.rounds ? cus : std::max<int64_t>(1, std::min(cus, tiles)));
+  p.per_split = int(nk);
+  if (rest) {
+    // Whole, one a workgroup; or dealt out, at least 8 k tiles each, with the
+    // sums' round trip (256 KB a part, by the memory's rate in k tiles' time).
+    const double whole = double(nk) + kEnds;
+    const int64_t per = std::max<int64_t>(8, ceil_div(rest * nk, cus));
+    const int64_t parts = ceil_div(rest * nk, per) + rest;
+    const double dealt = double(per) + 2 * kEnds + 6.0 + double(parts) * 0.1;
+    if (per < nk && dealt < whole) {
+      p.per_split = int(per);
+      if (!p.rounds) p.split = int(ceil_div(rest * nk, per));
+      p.partial_bytes = size_t(p.split + rest) * 256 * 256 * 4;
+      c += dealt;
+    } else {
+      c += whole;
+    }
+  }
+  *cost = c;
+  return p;
+}
+
+// A pointer into a workspace that is not there yet is null: its place is aligned.
+Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
+  const int64_t M = g.M, N = g.N, K = g.K;
+  const int nseg = g.nseg, npair = g.npair;
+  const bool gated = epi == kEpiGated;
+  const int kt = int(128 / elem_size(dtype));
+  const bool copyable = is_copyable(g, form, dtype, nseg == 2 || npair == 2 || gated);
+  Plan best{};
+  double best_cost = 0;
+  // The wide kernel has no fp32 form (fp32 products are bound by the matrix
+  // unit in either), takes whole words, and 32-bit offsets within 256 rows.
+  if (copyable && dtype != DN_F32 && K > 0 && g.lda < (1 << 23) && g.ldb < (1 << 23))
+    best = plan_wide(M, N, K, nseg, npair, dtype, gated, &best_cost);
+  Plan p{};
+  p.tile = kTile128;
+  p.tiles_m = int(ceil_div(M, 128));
+  p.tiles_n = int(ceil_div(N, gated ? 64 : 128));
+  p.ktiles = int(ceil_div(K, kt));
+  const int64_t ksteps = std::max<int64_t>(1, int64_t(p.ktiles) * nseg);
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair;
+  const int slots = device_cu_count() * 2;
+  const double unit = 0.72;  // a k tile's time on a full machine, to the wide kernel's
+  const int most = int(std::min<int64_t>(std::max<int64_t>(1, ksteps / 4), 64));
+  for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
+    const int64_t per = ceil_div(ksteps, s);
+    const int split = int(ceil_div(ksteps, per));
+    if (tiles * split > (int64_t(1) << 30)) break;
+    const double rounds = double(ceil_div(tiles * split, slots));
+    double cost = rounds * (double(per) + 6.0) * unit;
+    if (split > 1)  // partial sums out and in, at a CU's share of the memory's rate
+      cost += 6.0 + double(M) * N * (gated ? 2 : 1) * npair * split * 8.0 / 6.0e6;
+    if (best.split == 0 || cost < best_cost) {
+      best_cost = cost;
+      p.split = split;
+      p.per_split = int(per);
+      p.partial_bytes =
+          split > 1 ? align_up(size_t(split) * npair * size_t(M) *
+                                   size_t(gated ? 2 * N : align_up(size_t(N), 4)) * 4, 256)
+                    : 0;
+      best = p;
+    }
+    if (s > 1 && tiles * s >= 4 * int64_t(slots)) break;
+  }
+  best.copyable = copyable;
+  return best;
+}
+
+void apply(GemmArgs& g, const Plan& p, bool gated, float* partial) {
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.ktiles = p.ktiles;
+  g.split = p.split;
+  g.per_split = p.per_split;
+  g.rounds = p.rounds;
+  g.partial = p.partial_bytes ? partial : nullptr;
+  g.ldpart = gated ? 2 * int64_t(g.N) : int64_t(align_up(size_t(g.N), 4));
+}
+
+template <class TO, int EPI>
+hipError_t join_go(const GemmArgs& g, GemmTile tile, hipStream_t stream) {
+  if (tile == kTileWide) {
+    const int rest = g.tiles_m * g.tiles_n * g.npair - g.rounds * g.split;
+    const int rows = kJoinThreads / (EPI == kEpiGated ? 16 : 32);
+    hipLaunchKernelGGL((wide_join_kernel<TO, EPI>), dim3(unsigned(rest), unsigned(256 / rows)),
+                       dim3(kJoinThreads), 0, stream, g);
+  } else {
+    const int64_t n = int64_t(g.M) * ((g.N + 7) / 8) * g.npair;
+    hipLaunchKernelGGL((gemm_join_kernel<TO, EPI>), dim3(unsigned(ceil_div(n, kJoinThreads))),
+                       dim3(kJoinThreads), 0, stream, g);
+  }
   return hipGetLastError();
+}
+template <class TO>
+hipError_t join_typed(const GemmArgs& g, GemmEpi epi, GemmTile tile, hipStream_t stream) {
+  if (epi == kEpiLinear) return join_go<TO, kEpiLinear>(g, tile, stream);
+  if (epi == kEpiGated) return join_go<TO, kEpiGated>(g, tile, stream);
+  return join_go<TO, kEpiDGated>(g, tile, stream);
 }
 
 hipError_t run_product(GemmArgs& g, GemmForm form, GemmEpi epi, int dtype, int out_dtype,
                        const Plan& plan, float* partial, const char* name, hipStream_t stream) {
-  const bool gated = epi == kEpiGated;
-  apply(g, plan, gated, partial);
-  const bool staged = !copyable(g, form, dtype, g.nseg == 2 || g.npair == 2 || gated);
+  apply(g, plan, epi == kEpiGated, partial);
   hipError_t e;
   {
     ProfScope ps(name, stream);
     if (dtype == DN_F8) e = gemm_f8(g, out_dtype, plan.tile, stream);
-    else if (dtype == DN_BF16) e = gemm_bf16(g, form, epi, plan.tile, staged, stream);
-    else e = gemm_f32(g, form, epi, plan.tile, staged, stream);
+    else if (dtype == DN_BF16) e = gemm_bf16(g, form, epi, plan.tile, !plan.copyable, stream);
+    else e = gemm_f32(g, form, epi, plan.tile, !plan.copyable, stream);
   }
-  if (e != hipSuccess || plan.split == 1) return e;
+  if (e != hipSuccess || !plan.partial_bytes) return e;
   ProfScope ps("dn_product_join", stream);
-  return out_dtype == DN_BF16 ? join_typed<bf16>(g, epi, stream)
-                              : join_typed<float>(g, epi, stream);
+  return out_dtype == DN_BF16 ? join_typed<bf16>(g, epi, plan.tile, stream)
+                              : join_typed<float>(g, epi, plan.tile, stream);
 }
 
 // --- act' and the bias' gradient -------------------------------------------------
@@ -249,123 +345,74 @@ struct Carve {
   }
 };
 
-// --- dn_linear --------------------------------------------------------------------
-
-Plan linear_plan(const dn_linear_args& a) {
-  return plan_product(a.rows, a.out_dim, a.in_dim, 1, 1, a.dtype, false);
-}
-
-struct LinearBwd {
-  Plan dx, dw;
-  Strips strips;
-  int64_t lddz;
-  void* dz;
-  float *sums, *partial;
-  size_t bytes;
+// One product of an operation.
+struct Product {
+  GemmArgs g;
+  GemmForm form;
+  GemmEpi epi;
+  const char* name;
+  Plan plan;
 };
-LinearBwd linear_bwd_plan(const dn_linear_bwd_args& a, void* ws) {
-  LinearBwd p{};
-  size_t partial = 0;
-  if (a.d_x && a.rows > 0) {
-    p.dx = plan_product(a.rows, a.in_dim, a.out_dim, 1, 1, a.dtype, false);
-    partial = p.dx.partial_bytes;
-  }
-  if (a.d_weight) {
-    p.dw = plan_product(a.in_dim, a.out_dim, a.rows, 1, 1, a.dtype, false);
-    partial = std::max(partial, p.dw.partial_bytes);
-  }
-  Carve c{static_cast<char*>(ws)};
-  p.lddz = int64_t(align_up(size_t(a.out_dim), 16));
-  if (a.activation != DN_ACT_IDENTITY)
-    p.dz = c.take(size_t(a.rows) * size_t(p.lddz) * elem_size(a.dtype));
-  p.strips = strips_of(a.rows, a.out_dim);
-  if (a.d_bias) p.sums = static_cast<float*>(c.take(size_t(p.strips.count) * a.out_dim * 4));
-  if (partial) p.partial = static_cast<float*>(c.take(partial));
-  p.bytes = c.used;
-  return p;
-}
 
-// --- dn_gated_ffn -----------------------------------------------------------------
+// An operation's products, in order, and its workspace: what they share, then
+// room for the largest one's partial sums. Laid out the same with no workspace
+// given (`ws` null), to size it.
+struct Steps {
+  int dtype, out_dtype;
+  Carve carve;
+  Product product[4];
+  int count = 0;
+
+  // M × N over K: a (lda elements a row) times b.
+  GemmArgs& add(const char* name, GemmForm form, GemmEpi epi, int64_t M, int64_t N, int64_t K,
+                const void* a, int64_t lda, const void* b, int64_t ldb) {
+    const int64_t es = int64_t(elem_size(dtype));
+    Product& p = product[count++];
+    p = Product{};
+    p.form = form;
+    p.epi = epi;
+    p.name = name;
+    p.g.a[0] = static_cast<const char*>(a);
+    p.g.b[0] = static_cast<const char*>(b);
+    p.g.lda = lda * es;
+    p.g.ldb = ldb * es;
+    p.g.M = int(M);
+    p.g.N = int(N);
+    p.g.K = int(K);
+    p.g.nseg = p.g.npair = 1;
+    return p.g;
+  }
+  size_t finish() {
+    size_t partial = 0;
+    for (int i = 0; i < count; ++i) {
+      product[i].plan = plan_product(product[i].g, product[i].form, product[i].epi, dtype);
+      partial = std::max(partial, product[i].plan.partial_bytes);
+    }
+    partials = partial ? static_cast<float*>(carve.take(partial)) : nullptr;
+    return carve.used;
+  }
+  hipError_t run(hipStream_t stream) {
+    for (int i = 0; i < count; ++i) {
+      Product& p = product[i];
+      const hipError_t e = run_product(p.g, p.form, p.epi, dtype, out_dtype, p.plan, partials,
+                                       p.name, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
+  float* partials = nullptr;
+};
 
 int64_t padded(int64_t n) { return int64_t(align_up(size_t(n), 16)); }
 
-struct FfnFwd {
-  Plan in, down;
-  void* h;
-  float* partial;
-  size_t bytes;
-};
-FfnFwd ffn_plan(const dn_gated_ffn_args& a, void* ws) {
-  FfnFwd p{};
-  p.in = plan_product(a.rows, a.hidden, a.dim, 1, 1, a.dtype, true);
-  p.down = plan_product(a.rows, a.dim, a.hidden, 1, 1, a.dtype, false);
-  Carve c{static_cast<char*>(ws)};
-  p.h = c.take(size_t(a.rows) * size_t(padded(a.hidden)) * elem_size(a.dtype));
-  const size_t partial = std::max(p.in.partial_bytes, p.down.partial_bytes);
-  if (partial) p.partial = static_cast<float*>(c.take(partial));
-  p.bytes = c.used;
-  return p;
-}
-
-struct FfnBwd {
-  Plan dh, dx, dw_in, dw_down;
-  void *dg, *du, *h;
-  float* partial;
-  size_t bytes;
-};
-FfnBwd ffn_bwd_plan(const dn_gated_ffn_bwd_args& a, void* ws) {
-  FfnBwd p{};
-  if (a.rows > 0) p.dh = plan_product(a.rows, a.hidden, a.dim, 1, 1, a.dtype, false);
-  size_t partial = p.dh.partial_bytes;
-  if (a.d_x && a.rows > 0) {
-    p.dx = plan_product(a.rows, a.dim, a.hidden, 2, 1, a.dtype, false);
-    partial = std::max(partial, p.dx.partial_bytes);
-  }
-  if (a.d_w_gate) {
-    p.dw_in = plan_product(a.dim, a.hidden, a.rows, 1, 2, a.dtype, false);
-    partial = std::max(partial, p.dw_in.partial_bytes);
-  }
-  if (a.d_w_down) {
-    p.dw_down = plan_product(a.hidden, a.dim, a.rows, 1, 1, a.dtype, false);
-    partial = std::max(partial, p.dw_down.partial_bytes);
-  }
-  Carve c{static_cast<char*>(ws)};
-  const size_t one = size_t(a.rows) * size_t(padded(a.hidden)) * elem_size(a.dtype);
-  p.dg = c.take(one);
-  p.du = c.take(one);
-  p.h = c.take(one);
-  if (partial) p.partial = static_cast<float*>(c.take(partial));
-  p.bytes = c.used;
-  return p;
-}
-
-const char* bytes_of(const void* p) { return static_cast<const char*>(p); }
-
-GemmArgs product(int64_t M, int64_t N, int64_t K, const void* a, int64_t lda, const void* b,
-                 int64_t ldb, int dtype) {
-  GemmArgs g{};
-  const int64_t es = int64_t(elem_size(dtype));
-  g.a[0] = bytes_of(a);
-  g.b[0] = bytes_of(b);
-  g.lda = lda * es;
-  g.ldb = ldb * es;
-  g.M = int(M);
-  g.N = int(N);
-  g.K = int(K);
-  g.nseg = g.npair = 1;
-  return g;
-}
-
-}  // namespace
-
-size_t linear_workspace(const dn_linear_args& a) { return linear_plan(a).partial_bytes; }
-
-hipError_t launch_linear(const dn_linear_args& a, void* ws, hipStream_t stream) {
-  const Plan plan = linear_plan(a);
-  GemmArgs g = product(a.rows, a.out_dim, a.in_dim, a.x, a.x_stride, a.weight, a.weight_stride,
-                       a.dtype);
+size_t linear_steps(const dn_linear_args& a, void* ws, Steps& s) {
+  s.dtype = a.dtype;
+  s.out_dtype = a.out_dtype;
+  s.carve.at = static_cast<char*>(ws);
   // 8-bit rows are padded with zeros to whole words.
-  if (a.dtype == DN_F8) g.K = int(align_up(size_t(a.in_dim), 16));
+  const int64_t k = a.dtype == DN_F8 ? padded(a.in_dim) : a.in_dim;
+  GemmArgs& g = s.add("dn_linear", a.dtype == DN_F8 ? kFormNT : kFormNN, kEpiLinear, a.rows,
+                      a.out_dim, k, a.x, a.x_stride, a.weight, a.weight_stride);
   g.act = a.activation;
   g.out[0] = a.out;
   g.ldo = a.out_stride;
@@ -376,137 +423,175 @@ hipError_t launch_linear(const dn_linear_args& a, void* ws, hipStream_t stream) 
   g.ldp = a.preact_stride;
   g.row_scale = a.x_scale;
   g.col_scale = a.weight_scale;
-  return run_product(g, a.dtype == DN_F8 ? kFormNT : kFormNN, kEpiLinear, a.dtype, a.out_dtype, plan,
-                     static_cast<float*>(ws), "dn_linear", stream);
+  return s.finish();
 }
 
-size_t linear_bwd_workspace(const dn_linear_bwd_args& a) {
-  return linear_bwd_plan(a, nullptr).bytes;
-}
-
-hipError_t launch_linear_bwd(const dn_linear_bwd_args& a, void* ws, hipStream_t stream) {
-  const LinearBwd p = linear_bwd_plan(a, ws);
-  const void* dz = a.d_out;
-  int64_t lddz = a.d_out_stride;
-  hipError_t e;
-  if (p.dz || a.d_bias) {
-    ActBwdArgs b{};
-    b.d_out = a.d_out;
-    b.ldd = a.d_out_stride;
-    b.z = p.dz ? a.preact : nullptr;
-    b.ldz = a.preact_stride;
-    b.dz = p.dz;
-    b.lddz = p.lddz;
-    b.sums = p.sums;
-    b.M = int(a.rows);
-    b.N = int(a.out_dim);
-    b.rows_per = p.strips.rows_per;
-    b.act = a.activation;
-      e = a.dtype == DN_BF16 ? act_bwd<bf16>(b, p.strips, a.d_bias, stream)
-                           : act_bwd<float>(b, p.strips, a.d_bias, stream);
-    if (e != hipSuccess) return e;
-    if (p.dz) {
-      dz = p.dz;
-      lddz = p.lddz;
-    }
-  }
+struct LinearBwd {
+  Strips strips;
+  int64_t lddz;
+  void* dz;
+  float* sums;
+};
+size_t linear_bwd_steps(const dn_linear_bwd_args& a, void* ws, Steps& s, LinearBwd& l) {
+  s.dtype = s.out_dtype = a.dtype;
+  s.carve.at = static_cast<char*>(ws);
+  const bool act = a.activation != DN_ACT_IDENTITY;
+  l.strips = strips_of(a.rows, a.out_dim);
+  l.lddz = padded(a.out_dim);
+  l.dz = act ? s.carve.take(size_t(a.rows) * size_t(l.lddz) * elem_size(a.dtype)) : nullptr;
+  l.sums = a.d_bias
+               ? static_cast<float*>(s.carve.take(size_t(l.strips.count) * size_t(a.out_dim) * 4))
+               : nullptr;
+  const void* dz = act ? l.dz : a.d_out;
+  const int64_t lddz = act ? l.lddz : a.d_out_stride;
   if (a.d_x && a.rows > 0) {
-    GemmArgs g = product(a.rows, a.in_dim, a.out_dim, dz, lddz, a.weight, a.weight_stride, a.dtype);
+    GemmArgs& g = s.add("dn_linear_dx", kFormNT, kEpiLinear, a.rows, a.in_dim, a.out_dim, dz, lddz,
+                        a.weight, a.weight_stride);
     g.out[0] = a.d_x;
     g.ldo = a.d_x_stride;
-      if ((e = run_product(g, kFormNT, kEpiLinear, a.dtype, a.dtype, p.dx, p.partial, "dn_linear_dx",
-                         stream)) != hipSuccess)
-      return e;
   }
   if (a.d_weight) {
-    GemmArgs g = product(a.in_dim, a.out_dim, a.rows, a.x, a.x_stride, dz, lddz, a.dtype);
+    GemmArgs& g = s.add("dn_linear_dw", kFormTN, kEpiLinear, a.in_dim, a.out_dim, a.rows, a.x,
+                        a.x_stride, dz, lddz);
     g.out[0] = a.d_weight;
     g.ldo = a.out_dim;
-      if ((e = run_product(g, kFormTN, kEpiLinear, a.dtype, a.dtype, p.dw, p.partial, "dn_linear_dw",
-                         stream)) != hipSuccess)
-      return e;
   }
-  return hipSuccess;
+  return s.finish();
 }
 
-size_t gated_ffn_workspace(const dn_gated_ffn_args& a) { return ffn_plan(a, nullptr).bytes; }
-
-hipError_t launch_gated_ffn(const dn_gated_ffn_args& a, void* ws, hipStream_t stream) {
-  const FfnFwd p = ffn_plan(a, ws);
+size_t ffn_steps(const dn_gated_ffn_args& a, void* ws, Steps& s) {
+  s.dtype = s.out_dtype = a.dtype;
+  s.carve.at = static_cast<char*>(ws);
   const int64_t ldh = padded(a.hidden);
-  GemmArgs g = product(a.rows, a.hidden, a.dim, a.x, a.x_stride, a.w_gate, a.w_in_stride, a.dtype);
-  g.b[1] = bytes_of(a.w_up);
-  g.act = a.activation;
-  g.out[0] = p.h;
-  g.ldo = ldh;
-  g.preact = a.gate;
-  g.up = a.up;
-  g.ldp = a.kept_stride;
-  hipError_t e = run_product(g, kFormNN, kEpiGated, a.dtype, a.dtype, p.in, p.partial,
-                             "dn_gated_ffn_in", stream);
-  if (e != hipSuccess) return e;
-  g = product(a.rows, a.dim, a.hidden, p.h, ldh, a.w_down, a.w_down_stride, a.dtype);
-  g.out[0] = a.out;
-  g.ldo = a.out_stride;
-  g.residual = a.residual;
-  g.ldr = a.residual_stride;
-  return run_product(g, kFormNN, kEpiLinear, a.dtype, a.dtype, p.down, p.partial,
-                     "dn_gated_ffn_down", stream);
+  void* h = s.carve.take(size_t(a.rows) * size_t(ldh) * elem_size(a.dtype));
+  GemmArgs& in = s.add("dn_gated_ffn_in", kFormNN, kEpiGated, a.rows, a.hidden, a.dim, a.x,
+                       a.x_stride, a.w_gate, a.w_in_stride);
+  in.b[1] = static_cast<const char*>(a.w_up);
+  in.act = a.activation;
+  in.out[0] = h;
+  in.ldo = ldh;
+  in.preact = a.gate;
+  in.up = a.up;
+  in.ldp = a.kept_stride;
+  GemmArgs& down = s.add("dn_gated_ffn_down", kFormNN, kEpiLinear, a.rows, a.dim, a.hidden, h, ldh,
+                         a.w_down, a.w_down_stride);
+  down.out[0] = a.out;
+  down.ldo = a.out_stride;
+  down.residual = a.residual;
+  down.ldr = a.residual_stride;
+  return s.finish();
 }
 
-size_t gated_ffn_bwd_workspace(const dn_gated_ffn_bwd_args& a) {
-  return ffn_bwd_plan(a, nullptr).bytes;
-}
-
-hipError_t launch_gated_ffn_bwd(const dn_gated_ffn_bwd_args& a, void* ws, hipStream_t stream) {
-  const FfnBwd p = ffn_bwd_plan(a, ws);
+size_t ffn_bwd_steps(const dn_gated_ffn_bwd_args& a, void* ws, Steps& s) {
+  s.dtype = s.out_dtype = a.dtype;
+  s.carve.at = static_cast<char*>(ws);
   const int64_t ldh = padded(a.hidden);
-  GemmArgs g = product(a.rows, a.hidden, a.dim, a.d_out, a.d_out_stride, a.w_down, a.w_down_stride,
-                       a.dtype);
-  g.act = a.activation;
-  g.out[0] = p.dg;
-  g.out[1] = p.du;
-  g.h = p.h;
-  g.ldo = ldh;
-  g.preact = const_cast<void*>(a.gate);
-  g.up = const_cast<void*>(a.up);
-  g.ldp = a.kept_stride;
-  hipError_t e = hipSuccess;
-  if (a.rows > 0)
-    e = run_product(g, kFormNT, kEpiDGated, a.dtype, a.dtype, p.dh, p.partial, "dn_gated_ffn_dh",
-                    stream);
-  if (e != hipSuccess) return e;
+  const size_t one = size_t(a.rows) * size_t(ldh) * elem_size(a.dtype);
+  void* dg = s.carve.take(one);
+  void* du = s.carve.take(one);
+  void* h = s.carve.take(one);
+  if (a.rows > 0) {
+    GemmArgs& g = s.add("dn_gated_ffn_dh", kFormNT, kEpiDGated, a.rows, a.hidden, a.dim, a.d_out,
+                        a.d_out_stride, a.w_down, a.w_down_stride);
+    g.act = a.activation;
+    g.out[0] = dg;
+    g.out[1] = du;
+    g.h = h;
+    g.ldo = ldh;
+    g.preact = const_cast<void*>(a.gate);
+    g.up = const_cast<void*>(a.up);
+    g.ldp = a.kept_stride;
+  }
   if (a.d_x && a.rows > 0) {
-    g = product(a.rows, a.dim, a.hidden, p.dg, ldh, a.w_gate, a.w_in_stride, a.dtype);
-    g.a[1] = bytes_of(p.du);
-    g.b[1] = bytes_of(a.w_up);
+    GemmArgs& g = s.add("dn_gated_ffn_dx", kFormNT, kEpiLinear, a.rows, a.dim, a.hidden, dg, ldh,
+                        a.w_gate, a.w_in_stride);
+    g.a[1] = static_cast<const char*>(du);
+    g.b[1] = static_cast<const char*>(a.w_up);
     g.nseg = 2;
     g.out[0] = a.d_x;
     g.ldo = a.d_x_stride;
-      if ((e = run_product(g, kFormNT, kEpiLinear, a.dtype, a.dtype, p.dx, p.partial,
-                         "dn_gated_ffn_dx", stream)) != hipSuccess)
-      return e;
   }
   if (a.d_w_gate) {
-    g = product(a.dim, a.hidden, a.rows, a.x, a.x_stride, p.dg, ldh, a.dtype);
-    g.b[1] = bytes_of(p.du);
+    GemmArgs& g = s.add("dn_gated_ffn_dw_in", kFormTN, kEpiLinear, a.dim, a.hidden, a.rows, a.x,
+                        a.x_stride, dg, ldh);
+    g.b[1] = static_cast<const char*>(du);
     g.npair = 2;
     g.out[0] = a.d_w_gate;
     g.out[1] = a.d_w_up;
     g.ldo = a.hidden;
-      if ((e = run_product(g, kFormTN, kEpiLinear, a.dtype, a.dtype, p.dw_in, p.partial,
-                         "dn_gated_ffn_dw_in", stream)) != hipSuccess)
-      return e;
   }
   if (a.d_w_down) {
-    g = product(a.hidden, a.dim, a.rows, p.h, ldh, a.d_out, a.d_out_stride, a.dtype);
+    GemmArgs& g = s.add("dn_gated_ffn_dw_down", kFormTN, kEpiLinear, a.hidden, a.dim, a.rows, h,
+                        ldh, a.d_out, a.d_out_stride);
     g.out[0] = a.d_w_down;
     g.ldo = a.dim;
-      if ((e = run_product(g, kFormTN, kEpiLinear, a.dtype, a.dtype, p.dw_down, p.partial,
-                         "dn_gated_ffn_dw_down", stream)) != hipSuccess)
-      return e;
   }
-  return hipSuccess;
+  return s.finish();
+}
+
+}  // namespace
+
+size_t linear_workspace(const dn_linear_args& a) {
+  Steps s;
+  return linear_steps(a, nullptr, s);
+}
+
+hipError_t launch_linear(const dn_linear_args& a, void* ws, hipStream_t stream) {
+  Steps s;
+  linear_steps(a, ws, s);
+  return s.run(stream);
+}
+
+size_t linear_bwd_workspace(const dn_linear_bwd_args& a) {
+  Steps s;
+  LinearBwd l;
+  return linear_bwd_steps(a, nullptr, s, l);
+}
+
+hipError_t launch_linear_bwd(const dn_linear_bwd_args& a, void* ws, hipStream_t stream) {
+  Steps s;
+  LinearBwd l;
+  linear_bwd_steps(a, ws, s, l);
+  if ((l.dz && a.rows > 0) || l.sums) {
+    ActBwdArgs b{};
+    b.d_out = a.d_out;
+    b.ldd = a.d_out_stride;
+    b.z = l.dz ? a.preact : nullptr;
+    b.ldz = a.preact_stride;
+    b.dz = l.dz;
+    b.lddz = l.lddz;
+    b.sums = l.sums;
+    b.M = int(a.rows);
+    b.N = int(a.out_dim);
+    b.rows_per = l.strips.rows_per;
+    b.act = a.activation;
+    const hipError_t e = a.dtype == DN_BF16 ? act_bwd<bf16>(b, l.strips, a.d_bias, stream)
+                                            : act_bwd<float>(b, l.strips, a.d_bias, stream);
+    if (e != hipSuccess) return e;
+  }
+  return s.run(stream);
+}
+
+size_t gated_ffn_workspace(const dn_gated_ffn_args& a) {
+  Steps s;
+  return ffn_steps(a, nullptr, s);
+}
+
+hipError_t launch_gated_ffn(const dn_gated_ffn_args& a, void* ws, hipStream_t stream) {
+  Steps s;
+  ffn_steps(a, ws, s);
+  return s.run(stream);
+}
+
+size_t gated_ffn_bwd_workspace(const dn_gated_ffn_bwd_args& a) {
+  Steps s;
+  return ffn_bwd_steps(a, nullptr, s);
+}
+
+hipError_t launch_gated_ffn_bwd(const dn_gated_ffn_bwd_args& a, void* ws, hipStream_t stream) {
+  Steps s;
+  ffn_bwd_steps(a, ws, s);
+  return s.run(stream);
 }
 
 }  // namespace dn

@@ -5,7 +5,7 @@
 
 namespace dn {
 
-enum GemmTile { kTile256, kTile128 };
+enum GemmTile { kTileWide, kTile128 };  // gemm_wide_kernel; gemm_kernel, 128 × 128
 // Operand layouts of a product (gemm.hpp): x·W, dz·Wᵀ, xᵀ·dz.
 enum GemmForm { kFormNN, kFormNT, kFormTN };
 
