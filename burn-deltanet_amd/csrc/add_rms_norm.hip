@@ -349,23 +349,28 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const T* d_out, const T* s
   dw[int64_t(blockIdx.y) * dim + c] = t;
 }
 
-// d_γ: the workgroups' sums added in order, four lanes of a column taking
-// every fourth workgroup.
+// d_γ: the workgroups' sums added in order, 64 lanes of a column taking every
+// 64th workgroup, their sums by halves.
+constexpr int kSumCols = 16, kSumLanes = 64;
 template <class TW>
-__global__ __launch_bounds__(256) void norm_dw_sum_kernel(const float* dw, TW* out, int parts,
-                                                          int dim) {
-  __shared__ float lds[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), l = threadIdx.x >> 5;
+__global__ __launch_bounds__(kSumCols * kSumLanes) void norm_dw_sum_kernel(const float* dw, TW* out,
+                                                                           int parts, int dim) {
+  __shared__ float lds[kSumLanes][kSumCols];
+  const int x = threadIdx.x % kSumCols, l = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + x;
   float t = 0.f;
-  if (c < dim)
-    for (int i = l; i < parts; i += 8) t += dw[int64_t(i) * dim + c];
-  lds[l][threadIdx.x & 31] = t;
-  __syncthreads();
-  if (l == 0 && c < dim) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) t += lds[i][threadIdx.x];
-    st(out, size_t(c), t);
+  if (c < dim) {
+#pragma unroll 4
+    for (int i = l; i < parts; i += kSumLanes) t += dw[int64_t(i) * dim + c];
   }
+  lds[l][x] = t;
+  __syncthreads();
+#pragma unroll
+  for (int half = kSumLanes / 2; half; half >>= 1) {
+    if (l < half) lds[l][x] += lds[l + half][x];
+    __syncthreads();
+  }
+  if (l == 0 && c < dim) st(out, size_t(c), lds[0][x]);
 }
 
 // Waves to a row and chunks a lane: one wave where that leaves every CU
@@ -453,8 +458,8 @@ hipError_t bwd_go(NormBwdArgs p, void* d_weight, void* ws, hipStream_t stream) {
     parts = strips;
   }
   ProfScope ps("dn_add_rms_norm_dw_sum", stream);
-  hipLaunchKernelGGL((norm_dw_sum_kernel<TW>), dim3(unsigned((p.dim + 31) / 32)), dim3(256), 0,
-                     stream, static_cast<const float*>(dw), static_cast<TW*>(d_weight), parts, p.dim);
+  hipLaunchKernelGGL((norm_dw_sum_kernel<TW>), dim3(unsigned((p.dim + kSumCols - 1) / kSumCols)),
+                     dim3(kSumCols * kSumLanes), 0, stream, static_cast<const float*>(dw), static_cast<TW*>(d_weight), parts, p.dim);
   return hipGetLastError();
 }
 

@@ -186,7 +186,7 @@ Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, 
   p.ktiles = int(ceil_div(K, int64_t(128 / elem_size(dtype))));
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair, nk = int64_t(p.ktiles) * nseg;
   const int64_t cus = device_cu_count();
-  constexpr double kEnds = 8.0;
+  constexpr double kEnds = 9.0;
   p.rounds = int(tiles / cus);
   const int64_t rest = tiles - p.rounds * cus;
   double c = p.rounds * (double(nk) + kEnds);
@@ -220,6 +220,11 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   const int kt = int(128 / elem_size(dtype));
   const bool copyable = is_copyable(g, form, dtype, nseg == 2 || npair == 2 || gated);
   Plan best{};
+  if (M <= few_rows_most(epi) && N >= 4 && form == (dtype == DN_F8 ? kFormNT : kFormNN)) {
+    best.tile = kTileFew;
+    best.copyable = copyable;
+    return best;
+  }
   double best_cost = 0;
   // The wide kernel has no fp32 form (fp32 products are bound by the matrix
   // unit in either), takes whole words, and 32-bit offsets within 256 rows.
@@ -233,14 +238,14 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   const int64_t ksteps = std::max<int64_t>(1, int64_t(p.ktiles) * nseg);
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair;
   const int slots = device_cu_count() * 2;
-  const double unit = 0.72;  // a k tile's time on a full machine, to the wide kernel's
+  const double unit = 0.65;  // a k tile's time on a full machine, to the wide kernel's
   const int most = int(std::min<int64_t>(std::max<int64_t>(1, ksteps / 4), 64));
   for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
     const int64_t per = ceil_div(ksteps, s);
     const int split = int(ceil_div(ksteps, per));
     if (tiles * split > (int64_t(1) << 30)) break;
     const double rounds = double(ceil_div(tiles * split, slots));
-    double cost = rounds * (double(per) + 6.0) * unit;
+    double cost = rounds * (double(per) + 3.0) * unit;
     if (split > 1)  // partial sums out and in, at a CU's share of the memory's rate
       cost += 6.0 + double(M) * N * (gated ? 2 : 1) * npair * split * 8.0 / 6.0e6;
     if (best.split == 0 || cost < best_cost) {
@@ -297,7 +302,8 @@ hipError_t run_product(GemmArgs& g, GemmForm form, GemmEpi epi, int dtype, int o
   hipError_t e;
   {
     ProfScope ps(name, stream);
-    if (dtype == DN_F8) e = gemm_f8(g, out_dtype, plan.tile, stream);
+    if (plan.tile == kTileFew) e = few_rows(g, epi, dtype, out_dtype, plan.copyable, stream);
+    else if (dtype == DN_F8) e = gemm_f8(g, out_dtype, plan.tile, stream);
     else if (dtype == DN_BF16) e = gemm_bf16(g, form, epi, plan.tile, !plan.copyable, stream);
     else e = gemm_f32(g, form, epi, plan.tile, !plan.copyable, stream);
   }

@@ -5,7 +5,8 @@
 
 namespace dn {
 
-enum GemmTile { kTileWide, kTile128 };  // gemm_wide_kernel; gemm_kernel, 128 × 128
+// gemm_wide_kernel; gemm_kernel, 128 × 128; few_rows_kernel.
+enum GemmTile { kTileWide, kTile128, kTileFew };
 // Operand layouts of a product (gemm.hpp): x·W, dz·Wᵀ, xᵀ·dz.
 enum GemmForm { kFormNN, kFormNT, kFormTN };
 
@@ -15,6 +16,11 @@ hipError_t gemm_f32(const GemmArgs& g, GemmForm form, GemmEpi epi, GemmTile tile
                     hipStream_t stream);
 // dz·Wᵀ's form only, 16-byte rows.
 hipError_t gemm_f8(const GemmArgs& g, int out_dtype, GemmTile tile, hipStream_t stream);
+
+// Forwards of few rows (few_rows.hip): x·W, 8-bit x·Wᵀ, the gated pair.
+int few_rows_most(GemmEpi epi);
+hipError_t few_rows(const GemmArgs& g, GemmEpi epi, int dtype, int out_dtype, bool copyable,
+                    hipStream_t stream);
 
 hipError_t launch_add_rms_norm(const dn_add_rms_norm_args& a, hipStream_t stream);
 size_t add_rms_norm_bwd_workspace(const dn_add_rms_norm_bwd_args& a);
