@@ -340,13 +340,15 @@ __device__ inline uint32_t lds_address(const void* p) {
 // The XOR on a word's place. "row" tiles have rows of 8 words, two rows to
 // the banks' 256 bytes: the 16 rows of a fragment read meet 16 places.
 __device__ inline int swizzle_row(int row) { return (row >> 1) & 7; }
-// "col" tiles: k's rows are whole multiples of 256 bytes. bf16: a transposing
-// read takes 32 bytes of rows 8q + 4h + 0…3 for the lanes' four groups q; the
-// eight rows of a half wave get eight places. fp32: rows 4q + i, 64 bytes each.
-template <class T>
+// "col" tiles of R columns. bf16: a transposing read takes 32 bytes of rows
+// 8q + 4h + 0…3 for the lanes' four groups q, and the eight rows of a half wave
+// get eight places; k's rows are whole multiples of 256 bytes, or (R = 64) two
+// make one. fp32: rows 4q + i, 64 bytes each.
+template <class T, int R>
 __device__ inline int swizzle_col(int k) {
-  if constexpr (sizeof(T) == 2) return 2 * ((k & 3) | ((k >> 1) & 4));
-  else return 4 * ((k >> 2) & 3);
+  if constexpr (sizeof(T) == 4) return 4 * ((k >> 2) & 3);
+  else if constexpr (R == 64) return 2 * (((k >> 1) & 1) | ((k >> 2) & 2));
+  else return 2 * ((k & 3) | ((k >> 1) & 4));
 }
 
 // Which 16-byte word of an operand goes to word `L` of its tile.
@@ -357,7 +359,7 @@ __device__ inline void tile_word(int L, int& r, int& c) {
   if constexpr (COL) {
     constexpr int W = R / Elem<T>::kCh;
     r = L / W;
-    c = (L % W) ^ swizzle_col<T>(r);
+    c = (L % W) ^ swizzle_col<T, R>(r);
   } else {
     r = L >> 3;
     c = (L & 7) ^ swizzle_row(r);
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
       if constexpr (sizeof(T) == 2) {
         // Transposing reads: lane s of group q names row 8q + 4h + s/4, columns
         // 4(s%4)…+3 of the block, and receives column s of those four rows.
-        const int g = (s >> 2) | ((q & 1) << 2);
+        const int g = width == 64 ? (s >> 3) | ((q & 1) << 1) : (s >> 2) | ((q & 1) << 2);
         const char* at = tile + (32 * kk + 8 * q + (s >> 2)) * (width * 2) + ((blk ^ g) * 32) +
                          (s & 3) * 8;
         typedef __attribute__((address_space(3))) i16x4* P;
@@ -640,29 +642,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
   }
   __syncthreads();
 
-  // Epilogue: 32 rows of the wave at a time through its own LDS.
+  // Epilogue: 32 rows (16 where the wave has no more) at a time through its
+  // own LDS.
   constexpr int kLd = 68;  // floats a row: 64 and a pad
-  float* stage = reinterpret_cast<float*>(smem) + wave * 32 * kLd;
+  constexpr int kBlocks = MI < 2 ? MI : 2, kRows = 16 * kBlocks;
+  float* stage = reinterpret_cast<float*>(smem) + wave * kRows * kLd;
   const int row0 = m0 + wm * (BM / WM);
   const int col0 = n0 + wn * (EPI == kEpiGated ? 32 : 64);
 #pragma unroll
-  for (int half = 0; half < MI / 2; ++half) {
+  for (int half = 0; half < MI / kBlocks; ++half) {
 #pragma unroll
-    for (int ii = 0; ii < 2; ++ii)
+    for (int ii = 0; ii < kBlocks; ++ii)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const f32x4 a = acc[2 * half + ii][j];
+        const f32x4 a = acc[kBlocks * half + ii][j];
         *reinterpret_cast<float4*>(stage + (ii * 16 + s) * kLd + j * 16 + 4 * q) =
             make_float4(a[0], a[1], a[2], a[3]);
       }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     constexpr int kPer = EPI == kEpiGated ? 4 : 8;  // lanes to a row
-    constexpr int kIts = 32 * kPer / 64;
+    constexpr int kIts = kRows * kPer / 64;
     Tail<TO, EPI> tails[kIts];
     const int col = col0 + (lane % kPer) * 8, c = (lane % kPer) * 8;
     auto row_of = [&](int it) {
-      return int64_t(row0) + half * 32 + it * (64 / kPer) + lane / kPer;
+      return int64_t(row0) + half * kRows + it * (64 / kPer) + lane / kPer;
     };
 #pragma unroll
     for (int it = 0; it < kIts; ++it)
@@ -773,7 +777,7 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
       sub = (w * 4) >> 4;  // 16 KB subtiles: 1024 words, four of each thread
       const int l = L & 1023;
       r = l >> (CH == 8 ? 4 : 5);
-      c = (l & (128 / CH - 1)) ^ swizzle_col<T>(r);
+      c = (l & (128 / CH - 1)) ^ swizzle_col<T, 128>(r);
     } else {
       sub = 0;
       r = L >> 3;

@@ -26,6 +26,7 @@ hipError_t gemm_tile(const GemmArgs& g, GemmTile tile, hipStream_t stream) {
       return hipGetLastError();
     }
   }
+  if (tile == kTile64) return gemm_go<T, TO, ACOL, BCOL, 64, 64, 4, 1, EPI, STAGED>(g, stream);
   return gemm_go<T, TO, ACOL, BCOL, 128, 128, 2, 2, EPI, STAGED>(g, stream);
 }
 

@@ -175,8 +175,27 @@ bool is_copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
   return ok;
 }
 
+// What the kernels take, in us, from their measured times with all CUs busy:
+// `lone` for a k tile where a CU has one workgroup (its copies' latency), or
+// `each` for every workgroup of the CU (the matrix unit, LDS), whichever is
+// more; `ends` for a tile's start and end. fp32: the matrix unit's rate.
+struct Cost {
+  double lone, each, ends;
+  int most;  // workgroups of a CU at once
+};
+Cost cost_of(GemmTile tile, int dtype) {
+  if (tile == kTileWide) return dtype == DN_F8 ? Cost{3.2, 3.2, 15, 1} : Cost{1.65, 1.65, 15, 1};
+  if (tile == kTile128)
+    return dtype == DN_F32  ? Cost{1.75, 1.75, 3, 2}
+           : dtype == DN_F8 ? Cost{1.1, 1.0, 3, 2}
+                            : Cost{0.65, 0.54, 3, 2};
+  return dtype == DN_F32 ? Cost{0.6, 0.45, 3, 4}
+         : dtype == DN_F8 ? Cost{0.75, 0.3, 3, 4}
+                          : Cost{0.6, 0.2, 3, 4};
+}
+
 // The wide kernel: one workgroup a CU, whole tiles in rounds, the rest's k
-// tiles dealt out. In k tiles' time: a tile's start and end cost about 8.
+// tiles dealt out.
 Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, bool gated,
                double* cost) {
   Plan p{};
@@ -186,19 +205,20 @@ Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, 
   p.ktiles = int(ceil_div(K, int64_t(128 / elem_size(dtype))));
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair, nk = int64_t(p.ktiles) * nseg;
   const int64_t cus = device_cu_count();
-  constexpr double kEnds = 9.0;
+  const Cost t = cost_of(kTileWide, dtype);
   p.rounds = int(tiles / cus);
   const int64_t rest = tiles - p.rounds * cus;
-  double c = p.rounds * (double(nk) + kEnds);
+  double c = p.rounds * (double(nk) * t.each + t.ends);
   p.split = int(p.rounds ? cus : std::max<int64_t>(1, std::min(cus, tiles)));
   p.per_split = int(nk);
   if (rest) {
-    // Whole, one a workgroup; or dealt out, at least 8 k tiles each, with the
-    // sums' round trip (256 KB a part, by the memory's rate in k tiles' time).
-    const double whole = double(nk) + kEnds;
+    // Whole, one a workgroup; or dealt out, at least 8 k tiles each, with up to
+    // two parts a workgroup, the join and the sums' round trip (256 KB a part at
+    // 4 TB/s).
+    const double whole = double(nk) * t.each + t.ends;
     const int64_t per = std::max<int64_t>(8, ceil_div(rest * nk, cus));
     const int64_t parts = ceil_div(rest * nk, per) + rest;
-    const double dealt = double(per) + 2 * kEnds + 6.0 + double(parts) * 0.1;
+    const double dealt = double(per) * t.each + 2 * t.ends + 4 + double(parts) * 0.13;
     if (per < nk && dealt < whole) {
       p.per_split = int(per);
       if (!p.rounds) p.split = int(ceil_div(rest * nk, per));
@@ -217,9 +237,9 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   const int64_t M = g.M, N = g.N, K = g.K;
   const int nseg = g.nseg, npair = g.npair;
   const bool gated = epi == kEpiGated;
-  const int kt = int(128 / elem_size(dtype));
   const bool copyable = is_copyable(g, form, dtype, nseg == 2 || npair == 2 || gated);
   Plan best{};
+  // Few rows: up to 64 (gated 32) W's traffic binds, not the products.
   if (M <= few_rows_most(epi) && N >= 4 && form == (dtype == DN_F8 ? kFormNT : kFormNN)) {
     best.tile = kTileFew;
     best.copyable = copyable;
@@ -227,38 +247,44 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   }
   double best_cost = 0;
   // The wide kernel has no fp32 form (fp32 products are bound by the matrix
-  // unit in either), takes whole words, and 32-bit offsets within 256 rows.
+  // unit in any), takes whole words, and 32-bit offsets within 256 rows.
   if (copyable && dtype != DN_F32 && K > 0 && g.lda < (1 << 23) && g.ldb < (1 << 23))
     best = plan_wide(M, N, K, nseg, npair, dtype, gated, &best_cost);
-  Plan p{};
-  p.tile = kTile128;
-  p.tiles_m = int(ceil_div(M, 128));
-  p.tiles_n = int(ceil_div(N, gated ? 64 : 128));
-  p.ktiles = int(ceil_div(K, kt));
-  const int64_t ksteps = std::max<int64_t>(1, int64_t(p.ktiles) * nseg);
-  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair;
-  const int slots = device_cu_count() * 2;
-  const double unit = 0.65;  // a k tile's time on a full machine, to the wide kernel's
-  const int most = int(std::min<int64_t>(std::max<int64_t>(1, ksteps / 4), 64));
-  for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
-    const int64_t per = ceil_div(ksteps, s);
-    const int split = int(ceil_div(ksteps, per));
-    if (tiles * split > (int64_t(1) << 30)) break;
-    const double rounds = double(ceil_div(tiles * split, slots));
-    double cost = rounds * (double(per) + 3.0) * unit;
-    if (split > 1)  // partial sums out and in, at a CU's share of the memory's rate
-      cost += 6.0 + double(M) * N * (gated ? 2 : 1) * npair * split * 8.0 / 6.0e6;
-    if (best.split == 0 || cost < best_cost) {
-      best_cost = cost;
-      p.split = split;
-      p.per_split = int(per);
-      p.partial_bytes =
-          split > 1 ? align_up(size_t(split) * npair * size_t(M) *
-                                   size_t(gated ? 2 * N : align_up(size_t(N), 4)) * 4, 256)
-                    : 0;
-      best = p;
+  const int64_t cus = device_cu_count();
+  for (const GemmTile tile : {kTile128, kTile64}) {
+    const int b = tile == kTile128 ? 128 : 64;
+    const Cost t = cost_of(tile, dtype);
+    Plan p{};
+    p.tile = tile;
+    p.tiles_m = int(ceil_div(M, b));
+    p.tiles_n = int(ceil_div(N, gated ? b / 2 : b));
+    p.ktiles = int(ceil_div(K, int64_t(128 / elem_size(dtype))));
+    const int64_t ksteps = std::max<int64_t>(1, int64_t(p.ktiles) * nseg);
+    const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair;
+    const int most = int(std::min<int64_t>(std::max<int64_t>(1, ksteps / 2), 64));
+    for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
+      const int64_t per = ceil_div(ksteps, s);
+      const int split = int(ceil_div(ksteps, per));
+      if (tiles * split > (int64_t(1) << 30)) break;
+      const int64_t w = ceil_div(tiles * split, cus), left = w % t.most;
+      const auto turn = [&](int64_t n) {
+        return double(per) * std::max(t.lone, t.each * double(n)) + t.ends;
+      };
+      double cost = double(w / t.most) * turn(t.most) + (left ? turn(left) : 0.0);
+      if (split > 1)  // the join, and the partial sums out and in at 4 TB/s
+        cost += 4 + double(M) * N * (gated ? 2 : 1) * npair * split * 8.0 / 4.0e6;
+      if (best.split == 0 || cost < best_cost) {
+        best_cost = cost;
+        p.split = split;
+        p.per_split = int(per);
+        p.partial_bytes =
+            split > 1 ? align_up(size_t(split) * npair * size_t(M) *
+                                     size_t(gated ? 2 * N : align_up(size_t(N), 4)) * 4, 256)
+                      : 0;
+        best = p;
+      }
+      if (s > 1 && tiles * s >= 4 * t.most * cus) break;
     }
-    if (s > 1 && tiles * s >= 4 * int64_t(slots)) break;
   }
   best.copyable = copyable;
   return best;

@@ -56,10 +56,15 @@ class GatedFfnGrads(NamedTuple):
 F8 = torch.float8_e4m3fn
 
 
+# The current device's index, without torch.cuda.current_device()'s check that
+# CUDA is initialised: it is asked only about tensors that live there.
+_device = torch._C._cuda_getDevice
+
+
 def _gpu(t: Tensor, what: str) -> None:
     if not t.is_cuda:
         raise DeltaError(-6, f"{what}: tensors must live on the GPU (no CPU fallback)")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != _device():
         raise DeltaError(-6, f"{what}: lives on another GPU than the current one")
 
 
@@ -72,6 +77,8 @@ def _rows(t: Tensor, what: str) -> Tensor:
             raise DeltaError(-2, f"{what}: expected [..., dim], got a scalar")
         t = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty(
             (t.shape[:-1].numel(), t.shape[-1]))
+    if t.is_contiguous():
+        return t
     n, d = t.shape
     s0, s1 = t.stride()
     return t if (s1 == 1 or d == 1) and (n <= 1 or s0 >= d) else t.contiguous()
@@ -108,30 +115,45 @@ def _vector(v: Optional[Tensor], n: int, dtype, what: str) -> Optional[Tensor]:
 
 
 def _x_shape(x: Tensor) -> Tuple[int, int]:
+    if x.dim() == 2:
+        return x.shape
     if x.dim() == 0:
         raise DeltaError(-2, "x: expected [..., dim], got a scalar")
     return x.shape[:-1].numel(), x.shape[-1]
 
 
 def _grows(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _p(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _call(fn, args, size_fn, device) -> None:
+_ENTRIES = {}
+
+
+def _call(fn, args, sized, device) -> None:
     """The call on torch's current stream, with a workspace from torch's
     stream-ordered allocator where one is needed."""
-    L = abi.lib()
+    entry = _ENTRIES.get(fn)
+    if entry is None:
+        L = abi.lib()
+        entry = _ENTRIES[fn] = (getattr(L, fn), getattr(L, fn + "_workspace_bytes", None))
+    ref = ctypes.byref(args)
     ws = None
-    if size_fn is not None:
-        n = getattr(L, size_fn)(ctypes.byref(args))
+    if sized:
+        n = entry[1](ref)
         if n:
             ws = torch.empty(n, dtype=torch.uint8, device=device)
             args.workspace, args.workspace_bytes = ws.data_ptr(), n
-    abi.check(getattr(L, fn)(ctypes.byref(args), abi.stream_handle()))
+    rc = entry[0](ref, torch._C._cuda_getCurrentRawStream(_device()))
+    if rc:
+        abi.check(rc)
 
 
 # -- norm ----------------------------------------------------------------------
@@ -149,7 +171,7 @@ def _norm(x, residual, weight, eps, f8):
     a.x, a.x_stride, a.weight = x2.data_ptr(), x2.stride(0), w.data_ptr()
     total = x
     if r2 is not None:
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
         a.residual, a.residual_stride = r2.data_ptr(), r2.stride(0)
         a.sum, a.sum_stride = total.data_ptr(), dim
     scale = None
@@ -157,11 +179,12 @@ def _norm(x, residual, weight, eps, f8):
         out = torch.empty((rows, (dim + 15) // 16 * 16), dtype=F8, device=x.device)
         scale = torch.empty(rows, dtype=torch.float32, device=x.device)
         a.out, a.out_stride, a.scale = out.data_ptr(), out.stride(0), scale.data_ptr()
-        out = out[:, :dim]
+        if out.shape[1] != dim:
+            out = out[:, :dim]
     else:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         a.out, a.out_stride = out.data_ptr(), dim
-    _call("dn_add_rms_norm", a, None, x.device)
+    _call("dn_add_rms_norm", a, False, x.device)
     return out, scale, total
 
 
@@ -223,8 +246,7 @@ def add_rms_norm_backward(d_out: Tensor, d_sum: Optional[Tensor], total: Tensor,
     if ds is not None:
         a.d_sum, a.d_sum_stride = ds.data_ptr(), ds.stride(0)
     a.d_x, a.d_x_stride, a.d_weight = d_x.data_ptr(), dim, _p(d_w)
-    _call("dn_add_rms_norm_bwd", a, "dn_add_rms_norm_bwd_workspace_bytes" if need_weight else None,
-          total.device)
+    _call("dn_add_rms_norm_bwd", a, need_weight, total.device)
     return d_x, d_w
 
 
@@ -256,7 +278,7 @@ def _linear(x, weight, bias, activation, residual, keep):
     if keep and activation != Activation.IDENTITY:
         preact = torch.empty((rows, n), dtype=x.dtype, device=x.device)
         a.preact, a.preact_stride = preact.data_ptr(), n
-    _call("dn_linear", a, "dn_linear_workspace_bytes", x.device)
+    _call("dn_linear", a, True, x.device)
     return out, preact
 
 
@@ -320,7 +342,7 @@ def linear_backward(d_out: Tensor, x: Tensor, weight: Tensor, preact: Optional[T
     d_w = torch.empty((k, n), dtype=x.dtype, device=dev) if need_weight else None
     d_b = torch.empty(n, dtype=x.dtype, device=dev) if bias else None
     a.d_x, a.d_x_stride, a.d_weight, a.d_bias = _p(d_x), k, _p(d_w), _p(d_b)
-    _call("dn_linear_bwd", a, "dn_linear_bwd_workspace_bytes", dev)
+    _call("dn_linear_bwd", a, True, dev)
     return LinearGrads(d_x, d_w, d_b)
 
 
@@ -373,7 +395,7 @@ def linear_8bit(x: Rows8, weight: Rows8, bias: Optional[Tensor] = None,
         a.bias = b.data_ptr()
     if r is not None:
         a.residual, a.residual_stride = r.data_ptr(), r.stride(0)
-    _call("dn_linear", a, "dn_linear_workspace_bytes", c.device)
+    _call("dn_linear", a, True, c.device)
     return out
 
 
@@ -412,7 +434,7 @@ def _ffn(x, w_gate, w_up, w_down, activation, residual, keep):
         kept = torch.empty((2, rows, hidden), dtype=x.dtype, device=x.device)
         gate, up = kept[0], kept[1]
         a.gate, a.up, a.kept_stride = gate.data_ptr(), up.data_ptr(), hidden
-    _call("dn_gated_ffn", a, "dn_gated_ffn_workspace_bytes", x.device)
+    _call("dn_gated_ffn", a, True, x.device)
     return out, gate, up
 
 
@@ -479,5 +501,5 @@ def gated_ffn_backward(d_out: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w
     d_d = new((hidden, dim), need_down)
     a.d_x, a.d_x_stride = _p(d_x), dim
     a.d_w_gate, a.d_w_up, a.d_w_down = _p(d_g), _p(d_u), _p(d_d)
-    _call("dn_gated_ffn_bwd", a, "dn_gated_ffn_bwd_workspace_bytes", x.device)
+    _call("dn_gated_ffn_bwd", a, True, x.device)
     return GatedFfnGrads(d_x, d_g, d_u, d_d)
