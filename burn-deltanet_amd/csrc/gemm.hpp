@@ -368,24 +368,27 @@ __device__ inline void tile_word(int L, int& r, int& c) {
 
 }  // namespace gemm
 
-// BM × BN tiles, WM × WN waves. ACOL, BCOL: layouts. STAGED: operands whose
-// rows do not lie at 16-byte steps go through registers, with masks.
-template <class T, class TO, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, int EPI,
-          bool STAGED>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
+// BM × BN tiles, WM × WN parts of them, each of WK waves that share the k steps
+// of a tile; a ring of RING k tiles in LDS, RING − 1 in flight while one is
+// worked on. ACOL, BCOL: layouts. STAGED: operands whose rows do not lie at
+// 16-byte steps go through registers, with masks.
+template <class T, class TO, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, int WK,
+          int RING, int EPI, bool STAGED>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) {
   using namespace gemm;
   using E = Elem<T>;
-  constexpr int kThreads = 64 * WM * WN, CH = E::kCh, KT = E::kKT;
+  constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves, CH = E::kCh, KT = E::kKT;
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;  // 16×16 blocks of a wave
   constexpr int kABytes = BM * 128, kBBytes = BN * 128, kStage = kABytes + kBBytes;
   constexpr int NA = kABytes / 16 / kThreads, NB = kBBytes / 16 / kThreads;
   static_assert(NA * kThreads * 16 == kABytes && NB * kThreads * 16 == kBBytes, "whole copies");
   static_assert(NJ == 4, "the epilogue's rows of 64 columns");
-  __shared__ __attribute__((aligned(16))) char smem[2 * kStage];
+  static_assert(!STAGED || RING == 2, "one tile in the registers");
+  __shared__ __attribute__((aligned(16))) char smem[RING * kStage];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wk = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
   const int s = lane & 15, q = lane >> 4;
 
   // Workgroups go round the eight XCDs: each XCD gets a contiguous range of
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
 #pragma unroll
     for (int w = 0; w < NA; ++w) {
       int r, c;
-      tile_word<T, ACOL, BM>((w * WM * WN + wave) * 64 + lane, r, c);
+      tile_word<T, ACOL, BM>((w * kWaves + wave) * 64 + lane, r, c);
       if constexpr (ACOL)
         pa[w] = ga + int64_t(kt * KT + r) * p.lda +
                 int64_t(min(m0 + c * CH, p.M - CH)) * int(sizeof(T));
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
 #pragma unroll
     for (int w = 0; w < NB; ++w) {
       int r, c;
-      tile_word<T, BCOL, BN>((w * WM * WN + wave) * 64 + lane, r, c);
+      tile_word<T, BCOL, BN>((w * kWaves + wave) * 64 + lane, r, c);
       if constexpr (BCOL) {
         int which;
         const int col = min(b_col(c, which), p.N - CH);
@@ -496,7 +499,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
   auto masked_a = [&](int t, int w) {
     const int seg = t / p.ktiles, kt = t - seg * p.ktiles;
     int r, c;
-    tile_word<T, ACOL, BM>((w * WM * WN + wave) * 64 + lane, r, c);
+    tile_word<T, ACOL, BM>((w * kWaves + wave) * 64 + lane, r, c);
     const char* ga = seg ? p.a[1] : p.a[0];
     return ACOL ? masked(ga, p.lda, true, kt * KT + r, m0 + c * CH, p.M)
                 : masked(ga, p.lda, false, kt * KT + c * CH, m0 + r, p.M);
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
   auto masked_b = [&](int t, int w) {
     const int seg = t / p.ktiles, kt = t - seg * p.ktiles;
     int r, c, which = 0;
-    tile_word<T, BCOL, BN>((w * WM * WN + wave) * 64 + lane, r, c);
+    tile_word<T, BCOL, BN>((w * kWaves + wave) * 64 + lane, r, c);
     if constexpr (BCOL) {
       const int col = b_col(c, which);
       const char* gb = EPI == kEpiGated ? (which ? p.b[1] : p.b[0]) : (seg ? p.b[1] : gb0);
@@ -514,12 +517,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
     }
   };
   auto place = [&](int buf, int w, bool b) {
-    return smem + buf * kStage + (b ? kABytes : 0) + ((w * WM * WN + wave) * 64) * 16;
+    return smem + buf * kStage + (b ? kABytes : 0) + ((w * kWaves + wave) * 64) * 16;
   };
 
   // Tile t into buffer `buf`: copies in flight, or (STAGED, or a segment's
   // ragged last tile) through registers.
   uint4 ra[STAGED ? NA : 1], rb[STAGED ? NB : 1];
+  int kt = p.ktiles > 0 ? t0 % p.ktiles : 0;  // the next fetch's place in its segment
+  int plain = 0;                              // fetches by copies since the last other one
   auto fetch = [&](int t, int buf) {
     if constexpr (STAGED) {
 #pragma unroll
@@ -527,8 +532,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
 #pragma unroll
       for (int w = 0; w < NB; ++w) rb[w] = masked_b(t, w);
     } else {
-      const bool last = (t + 1) % p.ktiles == 0;
+      const bool last = ++kt == p.ktiles;
+      if (last) kt = 0;
+      ++plain;
       if (last && ragged) {
+        plain = 0;
 #pragma unroll
         for (int w = 0; w < NA; ++w)
           *reinterpret_cast<uint4*>(place(buf, w, false) + lane * 16) = masked_a(t, w);
@@ -615,17 +623,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
 
   if (t0 < t1) {
     if constexpr (!STAGED) sources(t0);
-    fetch(t0, 0);
+    int ready = t0;  // tiles fetched
+    for (; ready < min(t1, t0 + RING - 1); ++ready) fetch(ready, ready - t0);
     settle(0);
+    int buf = 0, fill = RING - 1;
     for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      wait_copies<0>();
-      __syncthreads();
-      if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+      // Tile t is there when no more copies are out than the RING − 2 tiles' after
+      // it, if those were all copied.
+      if (RING > 2 && ready - t == RING - 1 && plain >= RING - 2)
+        wait_copies<(RING - 2) * (NA + NB)>();
+      else
+        wait_copies<0>();
+      lds_barrier();
+      if (ready < t1) fetch(ready, fill);
       const char* ta = smem + buf * kStage;
       const char* tb = ta + kABytes;
 #pragma unroll
-      for (int kk = 0; kk < E::kSteps; ++kk) {
+      for (int kn = 0; kn < E::kSteps / WK; ++kn) {
+        const int kk = kn * WK + wk;
         Frag fb[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -637,20 +652,48 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs p) {
           for (int j = 0; j < NJ; ++j) mul(fb[j], fa, acc[i][j]);
         }
       }
-      if (t + 1 < t1) settle(buf ^ 1);
+      if (ready < t1) {
+        settle(fill);
+        ++ready;
+      }
+      fill = buf;
+      buf = buf + 1 == RING ? 0 : buf + 1;
     }
   }
   __syncthreads();
 
-  // Epilogue: 32 rows (16 where the wave has no more) at a time through its
-  // own LDS.
+  // The two waves of a part of the tile exchange sums: each keeps half of the
+  // row blocks, and adds in the order of the k steps.
+  constexpr int ME = MI / WK;
+  if constexpr (WK == 2) {
+    f32x4* mine = reinterpret_cast<f32x4*>(smem) + wave * ME * NJ * 64 + lane;
+    const f32x4* other =
+        reinterpret_cast<f32x4*>(smem) + (wave ^ (WM * WN)) * ME * NJ * 64 + lane;
+    static_assert(kWaves * ME * NJ * 1024 <= RING * kStage, "in LDS");
+#pragma unroll
+    for (int i = 0; i < ME; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) mine[(i * NJ + j) * 64] = wk ? acc[i][j] : acc[ME + i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ME; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const f32x4 v = other[(i * NJ + j) * 64];
+        acc[i][j] = wk ? v + acc[ME + i][j] : acc[i][j] + v;
+      }
+    __syncthreads();
+  }
+
+  // Epilogue: up to 32 rows of a wave at a time through its own LDS.
   constexpr int kLd = 68;  // floats a row: 64 and a pad
-  constexpr int kBlocks = MI < 2 ? MI : 2, kRows = 16 * kBlocks;
+  constexpr int kBlocks = ME < 2 || kWaves > 4 ? 1 : 2, kRows = 16 * kBlocks;
+  static_assert(kWaves * kRows * kLd * 4 <= RING * kStage, "in LDS");
   float* stage = reinterpret_cast<float*>(smem) + wave * kRows * kLd;
-  const int row0 = m0 + wm * (BM / WM);
+  const int row0 = m0 + wm * (BM / WM) + wk * (ME * 16);
   const int col0 = n0 + wn * (EPI == kEpiGated ? 32 : 64);
 #pragma unroll
-  for (int half = 0; half < MI / kBlocks; ++half) {
+  for (int half = 0; half < ME / kBlocks; ++half) {
 #pragma unroll
     for (int ii = 0; ii < kBlocks; ++ii)
 #pragma unroll

@@ -175,23 +175,34 @@ bool is_copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
   return ok;
 }
 
-// What the kernels take, in us, from their measured times with all CUs busy:
-// `lone` for a k tile where a CU has one workgroup (its copies' latency), or
-// `each` for every workgroup of the CU (the matrix unit, LDS), whichever is
-// more; `ends` for a tile's start and end. fp32: the matrix unit's rate.
+// What the kernels take, in us, from their measured times: `lone` for a k tile
+// where a CU has one workgroup, or `each` for every workgroup of the CU,
+// whichever is more; `ends` for a tile's start and end.
+//
+// kTile128: four waves of 64 x 64; two workgroups hide each other's waits.
+// kTileLone: the same tile by eight waves, two of them sharing each part's k
+// steps, for one workgroup a CU (bf16 1024 x 2048 x 4096 31 -> 25 us, 8-bit
+// 256 x 2048 x 12304 28 -> 22). kTile64: where 128 x 128 tiles are too few
+// (bf16 512 x 2048 x 4096: 18 us, kTileLone 24). Gated, its 32 columns of each
+// matrix are half lines of memory: 256 x 2048 x 5632 40 us, kTileLone 29.
 struct Cost {
   double lone, each, ends;
   int most;  // workgroups of a CU at once
 };
-Cost cost_of(GemmTile tile, int dtype) {
-  if (tile == kTileWide) return dtype == DN_F8 ? Cost{3.2, 3.2, 15, 1} : Cost{1.65, 1.65, 15, 1};
-  if (tile == kTile128)
-    return dtype == DN_F32  ? Cost{1.75, 1.75, 3, 2}
-           : dtype == DN_F8 ? Cost{1.1, 1.0, 3, 2}
-                            : Cost{0.65, 0.54, 3, 2};
-  return dtype == DN_F32 ? Cost{0.6, 0.45, 3, 4}
-         : dtype == DN_F8 ? Cost{0.75, 0.3, 3, 4}
-                          : Cost{0.6, 0.2, 3, 4};
+Cost cost_of(GemmTile tile, int dtype, bool gated) {
+  switch (tile) {
+    case kTileWide: return dtype == DN_F8 ? Cost{3.2, 3.2, 15, 1} : Cost{1.65, 1.65, 15, 1};
+    case kTile128:
+      return dtype == DN_F32  ? Cost{2.4, 2.1, 3, 2}
+             : dtype == DN_F8 ? Cost{1.55, 1.0, 3, 2}
+                              : Cost{0.85, 0.54, 3, 2};
+    case kTileLone: return dtype == DN_F8 ? Cost{1.15, 1.15, 4, 1} : Cost{0.65, 0.65, 4, 1};
+    default:
+      return dtype == DN_F32  ? Cost{0.8, 0.56, 3, 4}
+             : dtype == DN_F8 ? Cost{0.58, 0.27, 3, 4}
+             : gated          ? Cost{0.5, 0.36, 3, 3}
+                              : Cost{0.38, 0.22, 3, 3};
+  }
 }
 
 // The wide kernel: one workgroup a CU, whole tiles in rounds, the rest's k
@@ -205,7 +216,7 @@ Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, 
   p.ktiles = int(ceil_div(K, int64_t(128 / elem_size(dtype))));
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * npair, nk = int64_t(p.ktiles) * nseg;
   const int64_t cus = device_cu_count();
-  const Cost t = cost_of(kTileWide, dtype);
+  const Cost t = cost_of(kTileWide, dtype, gated);
   p.rounds = int(tiles / cus);
   const int64_t rest = tiles - p.rounds * cus;
   double c = p.rounds * (double(nk) * t.each + t.ends);
@@ -251,9 +262,10 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   if (copyable && dtype != DN_F32 && K > 0 && g.lda < (1 << 23) && g.ldb < (1 << 23))
     best = plan_wide(M, N, K, nseg, npair, dtype, gated, &best_cost);
   const int64_t cus = device_cu_count();
-  for (const GemmTile tile : {kTile128, kTile64}) {
-    const int b = tile == kTile128 ? 128 : 64;
-    const Cost t = cost_of(tile, dtype);
+  for (const GemmTile tile : {kTile128, kTileLone, kTile64}) {
+    if (tile == kTileLone && (!copyable || dtype == DN_F32)) continue;
+    const int b = tile == kTile64 ? 64 : 128;
+    const Cost t = cost_of(tile, dtype, gated);
     Plan p{};
     p.tile = tile;
     p.tiles_m = int(ceil_div(M, b));

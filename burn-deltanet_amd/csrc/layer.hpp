@@ -6,7 +6,7 @@
 namespace dn {
 
 // gemm_wide_kernel; gemm_kernel, 128 × 128 and 64 × 64; few_rows_kernel.
-enum GemmTile { kTileWide, kTile128, kTile64, kTileFew };
+enum GemmTile { kTileWide, kTile128, kTileLone, kTile64, kTileFew };
 // Operand layouts of a product (gemm.hpp): x·W, dz·Wᵀ, xᵀ·dz.
 enum GemmForm { kFormNN, kFormNT, kFormTN };
 
