@@ -136,8 +136,8 @@ __device__ inline void act8(const float (&z)[8], int kind, float (&a)[8], float 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = z[i];
-      a[i] = fmaxf(x, 0.f);
-      if constexpr (SLOPE) d[i] = x > 0.f ? 1.0f : 0.f;
+      a[i] = x < 0.f ? 0.f : x;  // NaN stays
+      if constexpr (SLOPE) d[i] = x <= 0.f ? 0.f : 1.0f;
     }
   } else {
 #pragma unroll

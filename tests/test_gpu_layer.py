@@ -155,6 +155,21 @@ def test_linear(rows, k, n, dtype):
             R.check(preact, (z, R.rounded(z, ez, T)), "preact")
 
 
+@pytest.mark.parametrize("rows", [2, 70])
+@pytest.mark.parametrize("kind", ACTS)
+def test_activations_keep_nan(rows, kind):
+    announce(f"linear {rows}x64x72 {kind}: NaN in a row")
+    g = gen(rows)
+    x, w = normal(g, rows, 64), normal(g, 64, 72)
+    x[1, 3] = math.nan
+    out, preact = dn.linear_forward(x, w, None, dn.Activation[kind.upper()])
+    assert torch.isnan(out[1]).all() and not torch.isnan(out[0]).any()
+    if preact is not None:
+        dx = dn.linear_backward(torch.ones_like(out), x, w, preact,
+                                dn.Activation[kind.upper()]).d_x
+        assert not torch.isnan(dx[0]).any()
+
+
 @pytest.mark.parametrize("rows,k,n", LINEAR_SHAPES)
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_linear_backward(rows, k, n, dtype):
