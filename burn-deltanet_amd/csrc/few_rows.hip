@@ -265,7 +265,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs 
   // are read into its L2 once.
   const int groups = gridDim.x, per = groups >> 3, rem = groups & 7, xcd = blockIdx.x & 7;
   const int c0 = (xcd * per + min(xcd, rem) + (blockIdx.x >> 3)) * kCols;
-  const int K = p.K, chunks = K / 32;  // whole ones
+  // Whole chunks of this workgroup's share of the contraction.
+  const int K = p.K, all = K / 32, lo = int(blockIdx.y) * p.per_split;
+  const int chunks = min(p.per_split, all - lo);
 
   // Sources of a lane's copies from chunk 0 (words past N: the last whole one's).
   constexpr int kLanesRow = kRow / 16, kRows = 64 / kLanesRow;  // rows of a copy
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs 
   const int mine = chunks > wave ? (chunks - wave + kFewWaves - 1) / kFewWaves : 0;
 #pragma unroll
   for (int d = 0; d < kRing; ++d)
-    if (d < mine) fetch(d, wave + d * kFewWaves);
+    if (d < mine) fetch(d, lo + wave + d * kFewWaves);
   for (int n = 0; n < mine; n += kRing) {
 #pragma unroll
     for (int d = 0; d < kRing; ++d) {
@@ -325,13 +327,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs 
       if (n + d + kRing < mine) {
         // The fragments are in registers before their place is refilled.
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        fetch(d, wave + (n + d + kRing) * kFewWaves);
+        fetch(d, lo + wave + (n + d + kRing) * kFewWaves);
       }
     }
   }
-  if (K % 32 && chunks % kFewWaves == wave) {
+  if (K % 32 && lo + chunks == all && chunks % kFewWaves == wave) {
     // The ragged last rows, element by element: what lies past K is zero.
-    const int k = chunks * 32 + 8 * q;
+    const int k = all * 32 + 8 * q;
     auto eight = [&](auto at) {
       uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -385,7 +387,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs 
   const int i = threadIdx.x, row = i / (kCols / 8), c8 = (i % (kCols / 8)) * 8;
   if (row >= p.M || row >= 16 || c0 + c8 >= p.N) return;
   Tail<bf16, EPI> tail;
-  tail_load<bf16, EPI>(p, row, c0 + c8, tail);
+  if (!p.partial) tail_load<bf16, EPI>(p, row, c0 + c8, tail);
   float v[8], u[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -393,12 +395,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs 
     v[e] = sums[0][0][c8 >> 4][row & 3][at];
     if constexpr (NP == 2) u[e] = sums[0][1][c8 >> 4][row & 3][at];
   }
-  tail_store<bf16, EPI>(p, 0, row, c0 + c8, v, u, tail);
+  finish8<bf16, EPI>(p, 0, blockIdx.y, row, c0 + c8, v, u, tail);
 }
 
 template <int CB, int EPI>
 hipError_t few_copy_launch(const GemmArgs& g, hipStream_t stream) {
-  hipLaunchKernelGGL((few_rows_copy_kernel<CB, EPI>), dim3(unsigned((g.N + 16 * CB - 1) / (16 * CB))),
+  hipLaunchKernelGGL((few_rows_copy_kernel<CB, EPI>),
+                     dim3(unsigned((g.N + 16 * CB - 1) / (16 * CB)), unsigned(g.split)),
                      dim3(64 * kFewWaves), 0, stream, g);
   return hipGetLastError();
 }
@@ -430,6 +433,26 @@ hipError_t few_go(const GemmArgs& g, GemmEpi epi, hipStream_t stream) {
 }
 
 }  // namespace
+
+// Parts of the contraction, each a workgroup's for its columns. Few columns
+// leave CUs without work, and a CU takes W's rows at 28 GB/s whatever its waves
+// do: more parts where that makes up for the join's 4.5 us. One row of
+// 5632 x 2048: 13.8 us whole, four parts 6.8 and their join 3.3.
+int few_rows_split(const GemmArgs& g, GemmEpi epi, int dtype, bool copyable) {
+  if (dtype != DN_BF16 || !copyable || g.M > 16 || epi != kEpiLinear) return 1;
+  const int cus = device_cu_count(), groups = (g.N + 31) / 32, chunks = g.K / 32;
+  const double alone = double(g.K) * 64 / 28e3;
+  int best = 1;
+  double least = alone;
+  for (int s = 2; s * groups <= cus && s * 2 * kFewWaves <= chunks; ++s) {
+    const double cost = alone / s + 4.5;
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
 
 int few_rows_most(GemmEpi epi) { return epi == kEpiGated ? 32 : epi == kEpiLinear ? 64 : 0; }
 

@@ -254,6 +254,12 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
   if (M <= few_rows_most(epi) && N >= 4 && form == (dtype == DN_F8 ? kFormNT : kFormNN)) {
     best.tile = kTileFew;
     best.copyable = copyable;
+    const int64_t chunks = K / 32;  // of 32 rows of W
+    best.per_split = int(ceil_div(std::max<int64_t>(1, chunks),
+                                  few_rows_split(g, epi, dtype, copyable)));
+    best.split = int(std::max<int64_t>(1, ceil_div(chunks, best.per_split)));
+    if (best.split > 1)
+      best.partial_bytes = align_up(size_t(best.split) * M * align_up(size_t(N), 4) * 4, 256);
     return best;
   }
   double best_cost = 0;

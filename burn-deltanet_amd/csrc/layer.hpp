@@ -19,6 +19,7 @@ hipError_t gemm_f8(const GemmArgs& g, int out_dtype, GemmTile tile, hipStream_t 
 
 // Forwards of few rows (few_rows.hip): x·W, 8-bit x·Wᵀ, the gated pair.
 int few_rows_most(GemmEpi epi);
+int few_rows_split(const GemmArgs& g, GemmEpi epi, int dtype, bool copyable);
 hipError_t few_rows(const GemmArgs& g, GemmEpi epi, int dtype, int out_dtype, bool copyable,
                     hipStream_t stream);
 

@@ -55,6 +55,19 @@ def test_linear_8bit_large(rows, k, n):
     R.check(dn.linear_8bit(xq, wq, b, dn.Activation.SILU), ref, "out")
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 5632, 2048), (16, 8200, 264), (7, 16424, 8), (2, 4096, 4096)])
+def test_linear_few_rows_of_a_long_contraction(rows, k, n):
+    announce(f"linear {rows}x{k}x{n}")
+    g = gen(rows + k)
+    x, w = normal(g, rows, k, dtype=BF), normal(g, k, n, dtype=BF, scale=k ** -0.5)
+    b, r = normal(g, n, dtype=BF), normal(g, rows, n, dtype=BF)
+    (z, ez), ref = R.linear(d(x), d(w), d(b), "silu", d(r), BF)
+    out, preact = dn.linear_forward(view(x), view(w), b, dn.Activation.SILU, view(r))
+    R.check(out, ref, "out")
+    R.check(preact, (z, R.rounded(z, ez, BF)), "preact")
+    assert torch.equal(dn.linear(x, w, b, dn.Activation.SILU, r), out)
+
+
 def test_gated_ffn_large():
     rows, dim, hidden = 4104, 8200, 4104
     announce(f"gated_ffn {rows}x{dim}x{hidden}")
