@@ -439,8 +439,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
 
   // Word w of thread's copies: its place in the tile and its source.
   const char *pa[NA], *pb[NB];
-  auto sources = [&](int t) {  // of k tile t
-    const int seg = t / p.ktiles, kt = t - seg * p.ktiles;
+  auto sources = [&](int seg, int kt) {  // of a segment's k tile
     const char* ga = seg ? p.a[1] : p.a[0];
 #pragma unroll
     for (int w = 0; w < NA; ++w) {
@@ -496,16 +495,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
     }
     return v;
   };
-  auto masked_a = [&](int t, int w) {
-    const int seg = t / p.ktiles, kt = t - seg * p.ktiles;
+  // The next fetch's segment, and its place in it.
+  int seg = p.ktiles > 0 ? t0 / p.ktiles : 0, kt = t0 - seg * p.ktiles;
+  auto masked_a = [&](int w) {
     int r, c;
     tile_word<T, ACOL, BM>((w * kWaves + wave) * 64 + lane, r, c);
     const char* ga = seg ? p.a[1] : p.a[0];
     return ACOL ? masked(ga, p.lda, true, kt * KT + r, m0 + c * CH, p.M)
                 : masked(ga, p.lda, false, kt * KT + c * CH, m0 + r, p.M);
   };
-  auto masked_b = [&](int t, int w) {
-    const int seg = t / p.ktiles, kt = t - seg * p.ktiles;
+  auto masked_b = [&](int w) {
     int r, c, which = 0;
     tile_word<T, BCOL, BN>((w * kWaves + wave) * 64 + lane, r, c);
     if constexpr (BCOL) {
@@ -523,34 +522,37 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
   // Tile t into buffer `buf`: copies in flight, or (STAGED, or a segment's
   // ragged last tile) through registers.
   uint4 ra[STAGED ? NA : 1], rb[STAGED ? NB : 1];
-  int kt = p.ktiles > 0 ? t0 % p.ktiles : 0;  // the next fetch's place in its segment
-  int plain = 0;                              // fetches by copies since the last other one
+  int plain = 0;  // fetches by copies since the last other one
   auto fetch = [&](int t, int buf) {
+    const bool last = kt + 1 == p.ktiles;
     if constexpr (STAGED) {
 #pragma unroll
-      for (int w = 0; w < NA; ++w) ra[w] = masked_a(t, w);
+      for (int w = 0; w < NA; ++w) ra[w] = masked_a(w);
 #pragma unroll
-      for (int w = 0; w < NB; ++w) rb[w] = masked_b(t, w);
+      for (int w = 0; w < NB; ++w) rb[w] = masked_b(w);
+    } else if (last && ragged) {
+      plain = 0;
+#pragma unroll
+      for (int w = 0; w < NA; ++w)
+        *reinterpret_cast<uint4*>(place(buf, w, false) + lane * 16) = masked_a(w);
+#pragma unroll
+      for (int w = 0; w < NB; ++w)
+        *reinterpret_cast<uint4*>(place(buf, w, true) + lane * 16) = masked_b(w);
     } else {
-      const bool last = ++kt == p.ktiles;
-      if (last) kt = 0;
       ++plain;
-      if (last && ragged) {
-        plain = 0;
 #pragma unroll
-        for (int w = 0; w < NA; ++w)
-          *reinterpret_cast<uint4*>(place(buf, w, false) + lane * 16) = masked_a(t, w);
+      for (int w = 0; w < NA; ++w) copy_to_lds(pa[w], lds_address(place(buf, w, false)));
 #pragma unroll
-        for (int w = 0; w < NB; ++w)
-          *reinterpret_cast<uint4*>(place(buf, w, true) + lane * 16) = masked_b(t, w);
-      } else {
-#pragma unroll
-        for (int w = 0; w < NA; ++w) copy_to_lds(pa[w], lds_address(place(buf, w, false)));
-#pragma unroll
-        for (int w = 0; w < NB; ++w) copy_to_lds(pb[w], lds_address(place(buf, w, true)));
-      }
+      for (int w = 0; w < NB; ++w) copy_to_lds(pb[w], lds_address(place(buf, w, true)));
+    }
+    ++kt;
+    if (last) {
+      kt = 0;
+      ++seg;
+    }
+    if constexpr (!STAGED) {
       if (last) {
-        if (t + 1 < t1) sources(t + 1);
+        if (t + 1 < t1) sources(seg, 0);
       } else {
 #pragma unroll
         for (int w = 0; w < NA; ++w) pa[w] += step_a;
@@ -622,7 +624,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
   };
 
   if (t0 < t1) {
-    if constexpr (!STAGED) sources(t0);
+    if constexpr (!STAGED) sources(seg, kt);
     int ready = t0;  // tiles fetched
     for (; ready < min(t1, t0 + RING - 1); ++ready) fetch(ready, ready - t0);
     settle(0);

@@ -141,14 +141,21 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
   p.sums[int64_t(blockIdx.y) * p.N + c] = t;
 }
 
+// The strips' sums: 64 columns a workgroup, four lanes to each, which meet in LDS.
 template <class T>
 __global__ __launch_bounds__(256) void strip_sum_kernel(const float* sums, T* out, int strips,
                                                         int n) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
   float t = 0.f;
-  for (int i = 0; i < strips; ++i) t += sums[int64_t(i) * n + c];
-  st(out, size_t(c), t);
+  if (c < n) {
+#pragma unroll 8
+    for (int i = lane; i < strips; i += 4) t += sums[int64_t(i) * n + c];
+  }
+  __shared__ float lds[4][64];
+  lds[lane][threadIdx.x & 63] = t;
+  __syncthreads();
+  if (lane == 0 && c < n) st(out, size_t(c), lds[0][threadIdx.x] + lds[1][threadIdx.x] +
+                                                 lds[2][threadIdx.x] + lds[3][threadIdx.x]);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -362,11 +369,12 @@ hipError_t run_product(GemmArgs& g, GemmForm form, GemmEpi epi, int dtype, int o
 struct Strips {
   int rows_per, count;
 };
-// Strips of rows: enough workgroups to fill the CUs, at least 32 rows each.
+// Strips of rows: enough workgroups to fill the CUs, at least 8 rows each, one for
+// a lane (of 32: 7.9 us in place of 5.2 at 500 x 1039 in fp32).
 Strips strips_of(int64_t M, int64_t N) {
   const int64_t across = ceil_div(N, 256);
   const int64_t want = std::max<int64_t>(1, 1024 / across);
-  const int64_t per = std::max<int64_t>(32, ceil_div(M, want));
+  const int64_t per = std::max<int64_t>(8, ceil_div(M, want));
   return {int(per), int(std::max<int64_t>(1, ceil_div(M, per)))};
 }
 
@@ -380,7 +388,7 @@ hipError_t act_bwd(const ActBwdArgs& a, const Strips& st, void* d_bias, hipStrea
     if (e != hipSuccess || !a.sums) return e;
   }
   ProfScope ps("dn_linear_bias_sum", stream);
-  hipLaunchKernelGGL((strip_sum_kernel<T>), dim3(unsigned(ceil_div(a.N, 256))), dim3(256), 0, stream,
+  hipLaunchKernelGGL((strip_sum_kernel<T>), dim3(unsigned(ceil_div(a.N, 64))), dim3(256), 0, stream,
                      static_cast<const float*>(a.sums), static_cast<T*>(d_bias), st.count, a.N);
   return hipGetLastError();
 }
