@@ -198,11 +198,11 @@ struct Cost {
 };
 Cost cost_of(GemmTile tile, int dtype, bool gated) {
   switch (tile) {
-    case kTileWide: return dtype == DN_F8 ? Cost{3.2, 3.2, 15, 1} : Cost{1.65, 1.65, 15, 1};
+    case kTileWide: return dtype == DN_F8 ? Cost{3.2, 3.2, 9, 1} : Cost{1.65, 1.65, 9, 1};
     case kTile128:
       return dtype == DN_F32  ? Cost{2.4, 2.1, 3, 2}
              : dtype == DN_F8 ? Cost{1.55, 1.0, 3, 2}
-                              : Cost{0.85, 0.54, 3, 2};
+                              : Cost{0.85, 0.58, 3, 2};
     case kTileLone: return dtype == DN_F8 ? Cost{1.15, 1.15, 4, 1} : Cost{0.65, 0.65, 4, 1};
     default:
       return dtype == DN_F32  ? Cost{0.8, 0.56, 3, 4}
@@ -231,12 +231,12 @@ Plan plan_wide(int64_t M, int64_t N, int64_t K, int nseg, int npair, int dtype, 
   p.per_split = int(nk);
   if (rest) {
     // Whole, one a workgroup; or dealt out, at least 8 k tiles each, with up to
-    // two parts a workgroup, the join and the sums' round trip (256 KB a part at
-    // 4 TB/s).
+    // two parts a workgroup (their ends, with fp32 sums to store, take longer than
+    // a tile's), the join and the sums' round trip (256 KB a part at 4 TB/s).
     const double whole = double(nk) * t.each + t.ends;
     const int64_t per = std::max<int64_t>(8, ceil_div(rest * nk, cus));
     const int64_t parts = ceil_div(rest * nk, per) + rest;
-    const double dealt = double(per) * t.each + 2 * t.ends + 4 + double(parts) * 0.13;
+    const double dealt = double(per) * t.each + 28 + 4 + double(parts) * 0.13;
     if (per < nk && dealt < whole) {
       p.per_split = int(per);
       if (!p.rounds) p.split = int(ceil_div(rest * nk, per));
