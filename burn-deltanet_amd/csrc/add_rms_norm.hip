@@ -13,6 +13,14 @@
 //
 // d_γ sums over the rows: a workgroup keeps its rows' sums in registers and
 // writes them once; a second kernel adds the workgroups' in order.
+//
+// The sum and all statistics are fp32. A bf16 sum that is handed out is rounded
+// once (it is the residual stream, and is read again as such); the forward
+// normalises the unrounded one, the backward starts from what was handed out.
+//
+// Measured, bf16: 32768 x 2048 with a residual 97 us (5.5 TB/s, a copy's rate),
+// its gradient 164 us (3.3 TB/s) and 6 for d_γ's sum; 256 x 2048 into 8 bits
+// 4.4 us.
 #include <algorithm>
 
 #include "gemm.hpp"

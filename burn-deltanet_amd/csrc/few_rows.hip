@@ -246,6 +246,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs p) {
 // 16·CB columns (gated: of both matrices), with x's 32 columns beside them, and
 // reads both back as fragments, W's transposed. kRing chunks are in flight, 6 to 8 KB
 // of W a wave; no wave waits for another before the sums meet.
+//
+// Measured, one row of bf16: 2048 x 12304 10.8 us (4.7 TB/s), the gated pair of
+// 2048 x 5632 13.2 (3.5), 5632 x 2048 in four parts 6.8 and the join's 3.3.
 template <int CB, int EPI>
 __global__ __launch_bounds__(64 * kFewWaves) void few_rows_copy_kernel(GemmArgs p) {
   using namespace gemm;

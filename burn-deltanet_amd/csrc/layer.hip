@@ -12,6 +12,12 @@
 // split the contraction; their fp32 sums meet in the workspace and a second
 // kernel adds them in order and runs the epilogue (no atomics: the results do
 // not depend on the order of arrival).
+//
+// Roundings of a bf16 feed-forward's backward: gate and up are kept in bf16 (in
+// fp32 they would be 738 MB at 16384 x 5632, and not kept they would cost the
+// largest product again), and the matrix unit takes h, d_gate and d_up in bf16.
+// The gradients are 0.0035 from a 64-bit result in the norm, where rounding the
+// result alone gives 0.0017. The forward rounds h the same way: 0.0019.
 #include <algorithm>
 
 #include "layer.hpp"
