@@ -286,14 +286,13 @@ __device__ inline void tail_store(const GemmArgs& p, int z, int64_t row, int col
     store8(static_cast<TO*>(p.h) + row * p.ldo + col, h, valid);
   }
 }
-// Whether the sums are stored as they are. The whole epilogue is 5 KB of code for
-// each of the rows that a kernel unrolls, more than the instruction cache holds:
-// such products go by a path of their own that is short (bf16 8192 x 2048 x 12304
-// 468 -> 408 us).
+// Whether the sums are stored as they are, or with a residual. The whole epilogue
+// is 5 KB of code for each of the rows that a kernel unrolls, more than the
+// instruction cache holds: such products go by a path of their own that is short
+// (bf16 8192 x 2048 x 12304 468 -> 408 us).
 template <int EPI>
 __device__ inline bool stored_as_they_are(const GemmArgs& p) {
-  return EPI == kEpiLinear && p.act == DN_ACT_IDENTITY && !p.bias && !p.residual && !p.preact &&
-         !p.row_scale;
+  return EPI == kEpiLinear && p.act == DN_ACT_IDENTITY && !p.bias && !p.preact && !p.row_scale;
 }
 // Both parts, or the sums of a split product to the workspace.
 template <class TO, int EPI>
@@ -1083,7 +1082,8 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
         if (slot_no < 0 && row < p.M && col < p.N) tail_load<TO, EPI>(p, row, col, tails[n]);
       }
     };
-    fetch(0);
+    const bool bare = stored_as_they_are<EPI>(p);
+    if (!bare) fetch(0);
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
@@ -1113,14 +1113,29 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
         store8(to, v, 8);
         if constexpr (EPI == kEpiGated) store8(to + 128, u, 8);
       }
-    } else if (stored_as_they_are<EPI>(p)) {
-#pragma unroll 4
-      for (int it = 0; it < kPer; ++it) {
-        float v[8], u[8];
-        take(it, v, u);
-        if (row0 + local(it) < p.M && col < p.N)
-          store8(static_cast<TO*>(z ? p.out[1] : p.out[0]) + (row0 + local(it)) * p.ldo + col, v,
-                 p.N - col);
+    } else if (bare) {
+#pragma unroll 1
+      for (int it = 0; it < kPer; it += 4) {
+        Raw8<TO> r[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int64_t row = row0 + local(it + n);
+          if (p.residual && row < p.M && col < p.N)
+            r[n].load(static_cast<const TO*>(p.residual) + row * p.ldr + col, p.N - col);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          float v[8], u[8];
+          take(it + n, v, u);
+          const int64_t row = row0 + local(it + n);
+          if (p.residual) {
+            r[n].get(u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += u[i];
+          }
+          if (row < p.M && col < p.N)
+            store8(static_cast<TO*>(z ? p.out[1] : p.out[0]) + row * p.ldo + col, v, p.N - col);
+        }
       }
     } else {
       // What the epilogue reads for eight rows is in flight at a time, the first
