@@ -1071,7 +1071,7 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
   auto flush = [&](auto half) {
     constexpr int kHalfRows = decltype(half)::value;
     constexpr int kPer = EPI == kEpiGated ? 8 : 16;  // lanes to a row
-    constexpr int kAtOnce = EPI == kEpiGated ? 4 : 8;
+    constexpr int kAtOnce = EPI == kEpiDGated ? 4 : 2;
     const int64_t row0 = m0 + wm * 128 + kHalfRows * 64;
     const int col = n0 + wn * (EPI == kEpiGated ? 64 : 128) + (lane % kPer) * 8;
     Tail<TO, EPI> tails[kAtOnce];
