@@ -780,7 +780,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
 // Bound by the matrix unit's clock and by what of the loop does not hide behind
 // it: a k tile takes 1.65 us on all CUs (1.3 PFLOP/s), a round of tiles 5 to 9 us
 // of ends. Measured, bf16: 16384 x 4096 x 2048 x·W 260 us (1057 TFLOP/s), its
-// gradients 240 to 260; 8192 x 2048 x 12304 400 (1032); the feed-forward of
+// gradients 465 together; 8192 x 2048 x 12304 400 (1032); the feed-forward of
 // 16384 x 2048 x 5632 925, its backward 2157. 8-bit: 3.2 us a k tile of 128, the
 // bf16 rate.
 template <class T, class TO, bool ACOL, bool BCOL, int EPI>
