@@ -226,7 +226,11 @@ struct NormBwdArgs {
 // With a = Σ d_out·γ·s and inv = (mean(s²) + ε)^−½, u = s·inv:
 // d_x = inv·(d_out·γ − u·inv·a/dim) + d_s. A workgroup walks rows blockIdx.x·R,
 // + gridDim.x·R, … (R rows at once) and its lanes keep their columns' Σ d_out·u.
-template <class T, class TW, int WPR, int NCH>
+// Rows too long for registers: where d_x lies on d_out, which d_γ's sum still has
+// to read, the statistics and d_x are launches of their own, before and after it
+// (4096 x 16384 in bf16 210 us, else 195).
+enum { kStats = 1, kGradient = 2, kBoth = 3 };
+template <class T, class TW, int WPR, int NCH, int DO = kBoth>
 __global__ __launch_bounds__(kNormThreads) void add_rms_norm_bwd_kernel(NormBwdArgs p) {
   constexpr int kLanes = 64 * WPR, R = 4 / WPR;
   __shared__ float red[2][2][4];
@@ -288,32 +292,39 @@ __global__ __launch_bounds__(kNormThreads) void add_rms_norm_bwd_kernel(NormBwdA
         if (col < dim) store8(dx + col, v, dim - col);
       }
     } else {
-      for (int col = lane * 8; col < dim; col += kLanes * 8) {
-        float vs[8], vd[8], vw[8];
-        load8(s + col, vs, dim - col);
-        load8(dy + col, vd, dim - col);
-        load8(weight + col, vw, dim - col);
+      float inv, c;
+      if constexpr (DO & kStats) {
+        for (int col = lane * 8; col < dim; col += kLanes * 8) {
+          float vs[8], vd[8], vw[8];
+          load8(s + col, vs, dim - col);
+          load8(dy + col, vd, dim - col);
+          load8(weight + col, vw, dim - col);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss = fmaf(vs[i], vs[i], ss);
-          a = fmaf(vd[i] * vw[i], vs[i], a);
+          for (int i = 0; i < 8; ++i) {
+            ss = fmaf(vs[i], vs[i], ss);
+            a = fmaf(vd[i] * vw[i], vs[i], a);
+          }
         }
+        ss = row_reduce<WPR, false>(ss, red[turn][0]);
+        a = row_reduce<WPR, false>(a, red[turn][1]);
+        inv = 1.0f / sqrtf(ss / float(dim) + p.eps);
+        c = a * inv * inv / float(dim);
+        if (lane == 0 && p.row) p.row[row] = make_float2(inv, c);
+      } else {
+        inv = p.row[row].x;
+        c = p.row[row].y;
       }
-      ss = row_reduce<WPR, false>(ss, red[turn][0]);
-      a = row_reduce<WPR, false>(a, red[turn][1]);
-      const float inv = 1.0f / sqrtf(ss / float(dim) + p.eps);
-      const float c = a * inv * inv / float(dim);
-      if (lane == 0 && p.row) p.row[row] = make_float2(inv, c);
-      for (int col = lane * 8; col < dim; col += kLanes * 8) {
-        float vs[8], vd[8], vw[8], ve[8] = {};
-        load8(s + col, vs, dim - col);
-        load8(dy + col, vd, dim - col);
-        load8(weight + col, vw, dim - col);
-        if (ds) load8(ds + col, ve, dim - col);
+      if constexpr (DO & kGradient)
+        for (int col = lane * 8; col < dim; col += kLanes * 8) {
+          float vs[8], vd[8], vw[8], ve[8] = {};
+          load8(s + col, vs, dim - col);
+          load8(dy + col, vd, dim - col);
+          load8(weight + col, vw, dim - col);
+          if (ds) load8(ds + col, ve, dim - col);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ve[i] += inv * (vd[i] * vw[i] - vs[i] * c);
-        store8(dx + col, ve, dim - col);
-      }
+          for (int i = 0; i < 8; ++i) ve[i] += inv * (vd[i] * vw[i] - vs[i] * c);
+          store8(dx + col, ve, dim - col);
+        }
     }
   }
   if constexpr (NCH > 0) {
@@ -426,6 +437,15 @@ int strip_count(int64_t rows) {
   return int(std::max<int64_t>(1, (rows + strip_rows(rows) - 1) / strip_rows(rows)));
 }
 
+// Whether two matrices' extents in memory have a byte in common.
+template <class T>
+bool meet(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t dim) {
+  if (rows == 0) return false;
+  const auto p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  const auto bytes = [&](int64_t ld) { return uintptr_t((rows - 1) * ld + dim) * sizeof(T); };
+  return p < q + bytes(ldb) && q < p + bytes(lda);
+}
+
 template <class T, class TW>
 hipError_t bwd_go(NormBwdArgs p, void* d_weight, void* ws, hipStream_t stream) {
   const Shape s = shape_of(p.rows, p.dim);
@@ -437,6 +457,7 @@ hipError_t bwd_go(NormBwdArgs p, void* d_weight, void* ws, hipStream_t stream) {
   if (d_weight && s.nch == 0)
     p.row = reinterpret_cast<float2*>(static_cast<char*>(ws) +
                                       align_up(size_t(strips) * p.dim * 4, 256));
+  const bool late = p.row && meet<T>(p.d_x, p.ldx, p.d_out, p.ldo, p.rows, p.dim);
   {
     ProfScope ps("dn_add_rms_norm_bwd", stream);
     if (s.wpr == 1 && s.nch == 1)
@@ -451,18 +472,29 @@ hipError_t bwd_go(NormBwdArgs p, void* d_weight, void* ws, hipStream_t stream) {
       hipLaunchKernelGGL((add_rms_norm_bwd_kernel<T, TW, 4, 2>), grid, block, 0, stream, p);
     else if (s.nch == 4)
       hipLaunchKernelGGL((add_rms_norm_bwd_kernel<T, TW, 4, 4>), grid, block, 0, stream, p);
+    else if (late)
+      hipLaunchKernelGGL((add_rms_norm_bwd_kernel<T, TW, 4, 0, kStats>), grid, block, 0, stream,
+                         p);
     else
       hipLaunchKernelGGL((add_rms_norm_bwd_kernel<T, TW, 4, 0>), grid, block, 0, stream, p);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !d_weight) return e;
   if (s.nch == 0) {
-    ProfScope ps("dn_add_rms_norm_dw", stream);
-    hipLaunchKernelGGL((norm_dw_kernel<T>), dim3(unsigned((p.dim + 255) / 256), unsigned(strips)),
-                       dim3(256), 0, stream, static_cast<const T*>(p.d_out),
-                       static_cast<const T*>(p.sum), static_cast<const float2*>(p.row), dw, p.ldo,
-                       p.lds, p.rows, p.dim, strip_rows(p.rows));
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+    {
+      ProfScope ps("dn_add_rms_norm_dw", stream);
+      hipLaunchKernelGGL((norm_dw_kernel<T>), dim3(unsigned((p.dim + 255) / 256), unsigned(strips)),
+                         dim3(256), 0, stream, static_cast<const T*>(p.d_out),
+                         static_cast<const T*>(p.sum), static_cast<const float2*>(p.row), dw, p.ldo,
+                         p.lds, p.rows, p.dim, strip_rows(p.rows));
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (late) {
+      ProfScope ps("dn_add_rms_norm_bwd", stream);
+      hipLaunchKernelGGL((add_rms_norm_bwd_kernel<T, TW, 4, 0, kGradient>), grid, block, 0, stream,
+                         p);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     parts = strips;
   }
   ProfScope ps("dn_add_rms_norm_dw_sum", stream);

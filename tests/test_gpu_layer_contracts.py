@@ -1,0 +1,111 @@
+"""What the header and the descriptions of the operators around the mixer
+promise beside their formulas: outputs that lie on inputs, 8-bit rows in the
+storage of wider ones, the shapes and orders of differentiation, sizes up to
+the stated limits. References and bounds as in layer_util."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import layer_util as R
+from test_gpu_layer import BF, DEV, F32, TYPES, d, dn, gen, inside, normal
+from gpu_util import announce
+
+pytestmark = pytest.mark.gpu
+abi = dn.abi
+F8 = torch.float8_e4m3fn
+
+
+def entry(name, struct, **fields):
+    """One call of a C entry with the library's own workspace; tensors are given
+    by their address and, as <name>_stride, the distance of their rows."""
+    a = struct()
+    for k, v in fields.items():
+        if isinstance(v, torch.Tensor):
+            setattr(a, k, v.data_ptr())
+            if hasattr(a, k + "_stride"):
+                setattr(a, k + "_stride", v.stride(0))
+        elif v is not None:
+            setattr(a, k, v)
+    abi.check(getattr(abi.lib(), name)(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+
+
+# -- outputs on inputs -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,dim", [(3, 300), (2100, 1000), (5, 2049), (3, 8192), (70, 8200),
+                                      (2, 20001)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("on", ["d_out", "d_sum"])
+def test_norm_gradient_on_its_inputs(rows, dim, dtype, on):
+    announce(f"dn_add_rms_norm_bwd {rows}x{dim} {dtype}: d_x on {on}")
+    g, T = gen(rows + dim), TYPES[dtype]
+    s, w = normal(g, rows, dim, dtype=T), normal(g, dim, dtype=T)
+    t = {"d_out": normal(g, rows, dim, dtype=T), "d_sum": normal(g, rows, dim, dtype=T)}
+    ref = R.norm_bwd(d(s), d(w), d(t["d_out"]), d(t["d_sum"]), 1e-5, T, T)
+    d_w = torch.empty_like(w)
+    entry("dn_add_rms_norm_bwd", abi.AddRmsNormBwdArgs, rows=rows, dim=dim, eps=1e-5,
+          dtype=abi.dtype_tag(T), weight_dtype=abi.dtype_tag(T), sum=s, weight=w, d_x=t[on],
+          d_weight=d_w, **t)
+    R.check(t[on], ref["d_x"], "d_x")
+    R.check(d_w, ref["d_weight"], "d_weight")
+
+
+@pytest.mark.parametrize("rows,dim", [(3, 300), (2100, 1000), (5, 2049), (3, 8192), (4, 8200)])
+@pytest.mark.parametrize("out", ["bf16", "f32", "f8"])
+@pytest.mark.parametrize("on", ["x", "residual"])
+def test_norm_sum_on_its_inputs(rows, dim, out, on):
+    announce(f"dn_add_rms_norm {rows}x{dim} into {out}: sum on {on}")
+    T = F32 if out == "f32" else BF
+    g = gen(rows + dim)
+    t = {"x": normal(g, rows, dim, dtype=T), "residual": normal(g, rows, dim, dtype=T)}
+    w = normal(g, dim, dtype=T)
+    s_ref, y_ref, _ = R.norm(d(t["x"]), d(t["residual"]), d(w), 1e-5, T)
+    if out == "f8":
+        rows8, _ = dn.add_rms_norm_8bit(t["x"], t["residual"], w)
+    pad = (dim + 15) // 16 * 16
+    y = torch.empty((rows, pad), dtype=F8 if out == "f8" else T, device=DEV)
+    scale = torch.empty(rows, device=DEV)
+    entry("dn_add_rms_norm", abi.AddRmsNormArgs, rows=rows, dim=dim, eps=1e-5,
+          dtype=abi.dtype_tag(T), weight_dtype=abi.dtype_tag(T),
+          out_dtype=abi.DN_F8 if out == "f8" else abi.dtype_tag(T), weight=w, out=y, scale=scale,
+          sum=t[on], **t)
+    R.check(t[on], s_ref, "sum")
+    if out == "f8":
+        assert torch.equal(y[:, :dim].view(torch.uint8), rows8.codes.view(torch.uint8))
+        assert torch.equal(scale, rows8.scale)
+    else:
+        R.check(y[:, :dim], y_ref, "out")
+
+
+# One shape for each kernel and for each way to split its contraction.
+@pytest.mark.parametrize("rows,k,n", [(1, 5632, 2048), (3, 72, 136), (40, 100, 70), (70, 72, 300),
+                                      (256, 2048, 264), (1000, 683, 250), (2568, 16392, 1800)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_on_its_residual(rows, k, n, dtype):
+    announce(f"dn_linear {rows}x{k}x{n} {dtype}: out on the residual")
+    g, T = gen(rows + k + n), TYPES[dtype]
+    x, w = normal(g, rows, k, dtype=T), normal(g, k, n, dtype=T, scale=k ** -0.5)
+    r = normal(g, rows, n, dtype=T)
+    want = dn.linear(x, w, None, dn.Activation.SILU, r)
+    tag = abi.dtype_tag(T)
+    entry("dn_linear", abi.LinearArgs, rows=rows, in_dim=k, out_dim=n, dtype=tag, out_dtype=tag,
+          activation=abi.DN_ACT_SILU, x=x, weight=w, residual=r, out=r)
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("rows,dim,hidden", [(1, 264, 520), (33, 64, 64), (300, 250, 683)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gated_ffn_on_its_residual(rows, dim, hidden, dtype):
+    announce(f"dn_gated_ffn {rows}x{dim}x{hidden} {dtype}: out on the residual")
+    g, T = gen(rows + dim + hidden), TYPES[dtype]
+    x, r = normal(g, rows, dim, dtype=T), normal(g, rows, dim, dtype=T)
+    wg, wu = (normal(g, dim, hidden, dtype=T, scale=dim ** -0.5) for _ in range(2))
+    wd = normal(g, hidden, dim, dtype=T, scale=hidden ** -0.5)
+    want = dn.gated_ffn(x, wg, wu, wd, residual=r)
+    entry("dn_gated_ffn", abi.GatedFfnArgs, rows=rows, dim=dim, hidden=hidden,
+          dtype=abi.dtype_tag(T), activation=abi.DN_ACT_SILU, x=x, w_gate=wg, w_up=wu,
+          w_in_stride=hidden, w_down=wd, residual=r, out=r)
+    assert torch.equal(r, want)
