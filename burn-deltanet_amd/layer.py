@@ -352,11 +352,16 @@ def quantize_rows(t: Tensor) -> Rows8:
     if t.dim() != 2:
         raise DeltaError(-2, f"quantize_rows: expected [rows, dim], got {list(t.shape)}")
     t = t.float()
-    rows, dim = t.shape
     scale = t.abs().amax(1) / 448.0
-    store = torch.zeros((rows, (dim + 15) // 16 * 16), dtype=F8, device=t.device)
-    store[:, :dim].copy_(torch.where(scale[:, None] > 0, t / scale[:, None], t).to(F8))
-    return Rows8(store[:, :dim], scale)
+    return Rows8(_padded(torch.where(scale[:, None] > 0, t / scale[:, None], t).to(F8)), scale)
+
+
+def _padded(codes: Tensor) -> Tensor:
+    """A copy in storage whose rows are padded with zeros to a multiple of 16."""
+    rows, dim = codes.shape
+    store = torch.zeros((rows, (dim + 15) // 16 * 16), dtype=F8, device=codes.device)
+    store[:, :dim].copy_(codes)
+    return store[:, :dim]
 
 
 def _codes(r: Rows8, what: str) -> Tensor:
@@ -366,6 +371,8 @@ def _codes(r: Rows8, what: str) -> Tensor:
     if c.dim() != 2:
         raise DeltaError(-2, f"{what}: expected [rows, dim] codes, got {list(c.shape)}")
     _gpu(c, what)
+    if c.stride(1) != 1 and c.shape[1] > 1:
+        c = _padded(c)
     return c
 
 

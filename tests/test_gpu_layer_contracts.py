@@ -109,3 +109,30 @@ def test_gated_ffn_on_its_residual(rows, dim, hidden, dtype):
           dtype=abi.dtype_tag(T), activation=abi.DN_ACT_SILU, x=x, w_gate=wg, w_up=wu,
           w_in_stride=hidden, w_down=wd, residual=r, out=r)
     assert torch.equal(r, want)
+
+
+# -- 8-bit rows in wider storage ----------------------------------------------------
+
+
+def compact(r, cols):
+    """The columns `cols` of 8-bit rows in storage of their own."""
+    part = r.codes[:, cols]
+    n, k = part.shape
+    store = torch.zeros((n, (k + 15) // 16 * 16), dtype=F8, device=DEV)
+    store[:, :k].copy_(part)
+    return dn.Rows8(store[:, :k], r.scale)
+
+
+EIGHT_BIT_SHAPES = [(1, 1000, 264), (16, 250, 130), (40, 100, 70), (70, 40, 72), (257, 683, 264),
+                    (300, 100, 1033), (1, 100, 3), (4104, 4100, 4104)]
+
+
+@pytest.mark.parametrize("rows,k,n", EIGHT_BIT_SHAPES)
+def test_linear_8bit_takes_codes_that_are_not_adjacent(rows, k, n):
+    announce(f"linear_8bit {rows}x{k}x{n}: every other column of wider codes")
+    g = gen(rows + k)
+    xq, wq = dn.quantize_rows(normal(g, rows, 2 * k)), dn.quantize_rows(normal(g, n, 2 * k))
+    other = slice(None, None, 2)
+    want = dn.linear_8bit(compact(xq, other), compact(wq, other))
+    assert torch.equal(dn.linear_8bit(dn.Rows8(xq.codes[:, other], xq.scale),
+                                      dn.Rows8(wq.codes[:, other], wq.scale)), want)
