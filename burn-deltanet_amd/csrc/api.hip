@@ -994,8 +994,8 @@ int check_linear(const dn_linear_args* a) {
       return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride >= padded;
     };
     if (!whole(a->x, a->x_stride) || !whole(a->weight, a->weight_stride))
-      return fail(DN_ERR_UNSUPPORTED, "8-bit rows must start at 16-byte boundaries and hold "
-                                      "zeros up to the next multiple of 16");
+      return fail(DN_ERR_UNSUPPORTED, "8-bit rows must start at 16-byte boundaries and be stored "
+                                      "up to the next multiple of 16");
   }
   return DN_OK;
 }

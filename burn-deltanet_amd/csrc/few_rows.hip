@@ -96,22 +96,34 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(GemmArgs p) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) __builtin_memcpy(&st.x[m], xr[m] + int64_t(k) * ES, 16);
   };
-  // The ragged last step: what lies past K is zero in both.
+  // The ragged last step: what lies past K is zero in both. 8-bit rows hold whole
+  // words, whose codes past K may be any.
   auto fetch_ragged = [&](Step& st) {
     const int k = whole * KS + q * KL;
-    fetch_w(st, k, K);
+    fetch_w(st, k, kF8 ? (K + KL - 1) / KL * KL : K);
 #pragma unroll
     for (int n = 0; n < NP; ++n)
 #pragma unroll
-      for (int r = 0; r < NW; ++r)
+      for (int r = 0; r < NW; ++r) {
+        if constexpr (kF8) {
+          uint4 v;
+          __builtin_memcpy(&v, st.w[n][r], 16);
+          v = first_codes(v, K - k);
+          __builtin_memcpy(st.w[n][r], &v, 16);
+        } else {
 #pragma unroll
-        for (int d = 0; d < kDw; ++d)
-          if (kF8 ? k >= K : k + r >= K) st.w[n][r][d] = 0;
+          for (int d = 0; d < kDw; ++d)
+            if (k + r >= K) st.w[n][r][d] = 0;
+        }
+      }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       u32x4 v = {0, 0, 0, 0};
-      if constexpr (kF8) {  // 8-bit rows hold whole words
-        if (k < K) __builtin_memcpy(&v, xr[m] + k, 16);
+      if constexpr (kF8) {
+        if (k < K) {
+          __builtin_memcpy(&v, xr[m] + k, 16);
+          v = __builtin_bit_cast(u32x4, first_codes(__builtin_bit_cast(uint4, v), K - k));
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < KL; ++e) {

@@ -102,6 +102,16 @@ __device__ inline Codes16 widen(const uint4& c) {
           make_uint4(two(c.z, L{}), two(c.z, H{}), two(c.w, L{}), two(c.w, H{}))};
 }
 
+// The first n of a word's sixteen codes, zeros behind them: a row's last word may
+// hold another matrix's columns, or NaN.
+__device__ inline uint4 first_codes(uint4 v, int n) {
+  auto part = [&](uint32_t u, int from) {
+    const int k = n - from;
+    return k >= 4 ? u : k > 0 ? u & ((1u << (8 * k)) - 1u) : 0u;
+  };
+  return make_uint4(part(v.x, 0), part(v.y, 4), part(v.z, 8), part(v.w, 12));
+}
+
 // f(0), …, f(N − 1) with compile-time arguments.
 template <int... I, class F>
 __device__ inline void each_of(std::integer_sequence<int, I...>, F f) {
@@ -505,6 +515,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
         for (int n = 0; n < 8; ++n) h[n] = minor + n < minor_end ? e[n] : 0u;
         v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16,
                        h[6] | h[7] << 16);
+      } else {  // 8-bit rows hold whole words
+        __builtin_memcpy(&v, src, 16);
+        v = first_codes(v, minor_end - minor);
       }
     }
     return v;
@@ -921,8 +934,10 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
     const int major = col ? k : i, minor = col ? i : k;
     const int major_end = col ? p.K : extent, minor_end = col ? extent : p.K;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (major < major_end && minor < minor_end)  // whole words: the widths are
+    if (major < major_end && minor < minor_end) {  // whole words, as the operands hold them
       v = *reinterpret_cast<const uint4*>(base + int64_t(major) * ldx + int64_t(minor) * ES);
+      if constexpr (ES == 1) v = first_codes(v, minor_end - minor);
+    }
     return v;
   };
   // A segment's ragged last tile, through registers with masks.

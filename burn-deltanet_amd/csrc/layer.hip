@@ -184,7 +184,7 @@ bool is_copyable(const GemmArgs& g, GemmForm form, int dtype, bool second) {
   if (second) ok = ok && at16(g.b[1]) && (g.nseg == 1 || at16(g.a[1]));
   if (acol) ok = ok && g.M % ch == 0;
   if (bcol) ok = ok && g.N % ch == 0;
-  if (!acol || !bcol) ok = ok && g.K % ch == 0;
+  if ((!acol || !bcol) && dtype != DN_F8) ok = ok && g.K % ch == 0;  // 8-bit rows do
   return ok;
 }
 
@@ -473,10 +473,8 @@ size_t linear_steps(const dn_linear_args& a, void* ws, Steps& s) {
   s.dtype = a.dtype;
   s.out_dtype = a.out_dtype;
   s.carve.at = static_cast<char*>(ws);
-  // 8-bit rows are padded with zeros to whole words.
-  const int64_t k = a.dtype == DN_F8 ? padded(a.in_dim) : a.in_dim;
   GemmArgs& g = s.add("dn_linear", a.dtype == DN_F8 ? kFormNT : kFormNN, kEpiLinear, a.rows,
-                      a.out_dim, k, a.x, a.x_stride, a.weight, a.weight_stride);
+                      a.out_dim, a.in_dim, a.x, a.x_stride, a.weight, a.weight_stride);
   g.act = a.activation;
   g.out[0] = a.out;
   g.ldo = a.out_stride;

@@ -34,7 +34,8 @@ class Activation(IntEnum):
 class Rows8(NamedTuple):
     """A matrix held in 8 bits: e4m3 `codes` [rows, dim] with one `scale` a row;
     row i stands for codes[i] * scale[i]. The codes are a view of storage whose
-    rows are padded with zeros to a multiple of 16."""
+    rows start at multiples of 16 bytes and are whole multiples of 16 long, or a
+    part of wider ones: what stands past `dim` is not used."""
 
     codes: Tensor
     scale: Tensor
@@ -371,8 +372,13 @@ def _codes(r: Rows8, what: str) -> Tensor:
     if c.dim() != 2:
         raise DeltaError(-2, f"{what}: expected [rows, dim] codes, got {list(c.shape)}")
     _gpu(c, what)
-    if c.stride(1) != 1 and c.shape[1] > 1:
-        c = _padded(c)
+    rows, dim = c.shape
+    if c.stride(1) != 1 and dim > 1:
+        return _padded(c)
+    # A row's last word is read whole, the last row's too.
+    if dim % 16 and rows and (c.storage_offset() + (rows - 1) * c.stride(0) + (dim + 15) // 16 * 16
+                              > c.untyped_storage().nbytes()):
+        raise DeltaError(-9, f"{what}: 8-bit rows must be stored up to the next 16-byte boundary")
     return c
 
 

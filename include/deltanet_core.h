@@ -422,7 +422,7 @@ int dn_block_step(const dn_block_step_args *args, hipStream_t stream);
  * `dim` values, from the unrounded sum. With out_dtype DN_F8: scale[row] =
  * max|out| / 448, out = the e4m3 codes of out / scale (0 where the row is all
  * zeros), and the codes from `dim` up to the next multiple of 16 that fits in
- * out_stride are zero, as dn_linear's 8-bit operands need them. */
+ * out_stride are zero. */
 typedef struct {
   int64_t rows, dim;
   int64_t x_stride, residual_stride, sum_stride, out_stride;
@@ -462,9 +462,10 @@ size_t dn_add_rms_norm_bwd_workspace_bytes(const dn_add_rms_norm_bwd_args *args)
 
 /* out = act(x weight + bias) + residual, weight [in_dim, out_dim]. With dtype
  * DN_F8: x [rows, in_dim] and weight [out_dim, in_dim] are e4m3 codes with one
- * scale a row, the product is x_scale[row] * weight_scale[column] * (x weight^T),
- * and both strides are multiples of 16 bytes with zero codes from in_dim up to
- * the next multiple of 16. activation: DN_ACT_IDENTITY, SILU, RELU or GELU. */
+ * scale a row, the product is x_scale[row] * weight_scale[column] * (x weight^T).
+ * Both start at a multiple of 16 bytes, both strides are one, and every row, the
+ * last too, is stored up to the next multiple of 16 past in_dim: what stands
+ * there is read and not used. activation: DN_ACT_IDENTITY, SILU, RELU or GELU. */
 typedef struct {
   int64_t rows, in_dim, out_dim;
   int64_t x_stride, weight_stride, residual_stride, out_stride, preact_stride;

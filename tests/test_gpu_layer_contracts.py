@@ -136,3 +136,33 @@ def test_linear_8bit_takes_codes_that_are_not_adjacent(rows, k, n):
     want = dn.linear_8bit(compact(xq, other), compact(wq, other))
     assert torch.equal(dn.linear_8bit(dn.Rows8(xq.codes[:, other], xq.scale),
                                       dn.Rows8(wq.codes[:, other], wq.scale)), want)
+
+
+@pytest.mark.parametrize("rows,k,n", EIGHT_BIT_SHAPES)
+def test_linear_8bit_takes_a_part_of_wider_codes(rows, k, n):
+    """What stands beside the part, numbers or NaN, is not multiplied."""
+    announce(f"linear_8bit {rows}x{k}x{n}: columns 16 on of wider codes")
+    g = gen(rows + k + 1)
+    xq, wq = (dn.quantize_rows(normal(g, m, k + 40)) for m in (rows, n))
+    part = slice(16, 16 + k)
+    want = dn.linear_8bit(compact(xq, part), compact(wq, part))
+    for beside in (None, math.nan):
+        if beside is not None:
+            xq.codes[:, 16 + k:] = beside
+            wq.codes[:, 16 + k:] = beside
+        got = dn.linear_8bit(dn.Rows8(xq.codes[:, part], xq.scale),
+                             dn.Rows8(wq.codes[:, part], wq.scale))
+        assert torch.equal(got, want)
+
+
+def test_linear_8bit_refuses_rows_whose_storage_ends_early():
+    announce("linear_8bit: storage that ends inside the last word")
+    g = gen(3)
+    store = dn.quantize_rows(normal(g, 4, 48)).codes.flatten()
+    short = torch.empty(3 * 48 + 40, dtype=torch.uint8, device=DEV).view(F8)
+    short.copy_(store[:short.numel()])
+    codes = short.as_strided((4, 40), (48, 1))
+    w = dn.quantize_rows(normal(g, 72, 40))
+    with pytest.raises(dn.DeltaError, match="16-byte") as e:
+        dn.linear_8bit(dn.Rows8(codes, torch.ones(4, device=DEV)), w)
+    assert e.value.code == -9
