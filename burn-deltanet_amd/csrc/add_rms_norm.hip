@@ -85,9 +85,9 @@ __device__ inline uint2 codes8(const float (&v)[8], float scale) {
   return make_uint2(uint32_t(lo), uint32_t(hi));
 }
 // Codes of columns [col, col + 8), and zeros up to the next multiple of 16
-// where the row's storage holds them.
+// where the row's storage holds them (a lone row's stride may be any).
 __device__ inline void store_codes(uint8_t* row, int64_t ld, int col, int dim, const uint2& u) {
-  const int end = min(int64_t((dim + 15) & ~15), ld);
+  const int end = max(int64_t(dim), min(int64_t((dim + 15) & ~15), ld));
   if (col + 8 <= end) {
     __builtin_memcpy(row + col, &u, 8);
   } else {

@@ -166,3 +166,18 @@ def test_linear_8bit_refuses_rows_whose_storage_ends_early():
     with pytest.raises(dn.DeltaError, match="16-byte") as e:
         dn.linear_8bit(dn.Rows8(codes, torch.ones(4, device=DEV)), w)
     assert e.value.code == -9
+
+
+@pytest.mark.parametrize("stride", [0, 3, 40, 41, 48])
+def test_norm_8bit_of_one_row_needs_no_stride(stride):
+    announce(f"dn_add_rms_norm into 8 bits, one row, out_stride {stride}")
+    g = gen(4)
+    x, w = normal(g, 1, 40), normal(g, 40)
+    want, _ = dn.add_rms_norm_8bit(x, None, w)
+    y, scale = torch.full((48,), 1.0, device=DEV).to(F8), torch.empty(1, device=DEV)
+    entry("dn_add_rms_norm", abi.AddRmsNormArgs, rows=1, dim=40, eps=1e-5, out_dtype=abi.DN_F8,
+          x=x, weight=w, out=y.data_ptr(), out_stride=stride, scale=scale)
+    assert torch.equal(y[:40].view(torch.uint8), want.codes[0].view(torch.uint8))
+    got = y[40:].float()
+    filled = max(0, stride - 40)
+    assert not got[:filled].any() and (got[filled:] == 1.0).all()
