@@ -38,6 +38,7 @@ struct NormArgs {
   float* scale;
   int64_t ldx, ldr, lds, ldo;
   int rows, dim;
+  int end;  // of a row of codes
   float eps;
 };
 
@@ -84,10 +85,14 @@ __device__ inline uint2 codes8(const float (&v)[8], float scale) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(c[6], c[7], hi, true);
   return make_uint2(uint32_t(lo), uint32_t(hi));
 }
-// Codes of columns [col, col + 8), and zeros up to the next multiple of 16
-// where the row's storage holds them (a lone row's stride may be any).
-__device__ inline void store_codes(uint8_t* row, int64_t ld, int col, int dim, const uint2& u) {
-  const int end = max(int64_t(dim), min(int64_t((dim + 15) & ~15), ld));
+// Codes of columns [col, col + 8) of those before dim, and zeros up to `end`.
+__device__ inline void store_codes(uint8_t* row, int end, int col, int dim, uint2 u) {
+  if (col + 8 > dim) {
+    // Past dim 0 / scale is NaN in a row with a value that is not finite.
+    const int n = max(dim - col, 0);
+    const uint64_t c = (uint64_t(u.y) << 32 | u.x) & ((uint64_t(1) << (8 * n)) - 1);
+    u = make_uint2(uint32_t(c), uint32_t(c >> 32));
+  }
   if (col + 8 <= end) {
     __builtin_memcpy(row + col, &u, 8);
   } else {
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(kNormThreads) void add_rms_norm_kernel(NormArgs p) 
   };
   auto write = [&](int col, const float (&v)[8], float scale) {
     if constexpr (F8)
-      store_codes(static_cast<uint8_t*>(p.out) + row * p.ldo, p.ldo, col, dim, codes8(v, scale));
+      store_codes(static_cast<uint8_t*>(p.out) + row * p.ldo, p.end, col, dim, codes8(v, scale));
     else
       store8(static_cast<T*>(p.out) + row * p.ldo + col, v, dim - col);
   };
@@ -525,6 +530,9 @@ hipError_t launch_add_rms_norm(const dn_add_rms_norm_args& a, hipStream_t stream
   p.ldo = a.out_stride;
   p.rows = int(a.rows);
   p.dim = int(a.dim);
+  // Zeros up to the next multiple of 16 where the row's storage holds them (a lone
+  // row's stride may be any).
+  p.end = int(std::max(a.dim, std::min(int64_t(align_up(size_t(a.dim), 16)), a.out_stride)));
   p.eps = float(a.eps);
   ProfScope ps("dn_add_rms_norm", stream);
   const bool wb = a.weight_dtype == DN_BF16, f8out = a.out_dtype == DN_F8;

@@ -181,3 +181,14 @@ def test_norm_8bit_of_one_row_needs_no_stride(stride):
     got = y[40:].float()
     filled = max(0, stride - 40)
     assert not got[:filled].any() and (got[filled:] == 1.0).all()
+
+
+@pytest.mark.parametrize("dim", [7, 250, 2049, 8201])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_norm_8bit_pads_non_finite_rows_with_zeros_too(dim, bad):
+    announce(f"add_rms_norm_8bit 3x{dim}: {bad} in a row")
+    x = normal(gen(dim), 3, dim)
+    x[1, dim - 1] = bad
+    codes = dn.add_rms_norm_8bit(x, None, torch.ones(dim, device=DEV))[0].codes
+    pad = (dim + 15) // 16 * 16
+    assert not codes.as_strided((3, pad), (pad, 1)).view(torch.uint8)[:, dim:].any()
