@@ -79,6 +79,12 @@ __device__ inline uint2 codes8(const float (&v)[8], float scale) {
   float c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) c[i] = scale == 0.f ? v[i] : v[i] / scale;
+  // A denormal scale has few bits, and the row's largest value may be up to 1.5 times
+  // what 448 stands for, which the conversion makes NaN.
+  if (scale < 0x1p-126f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = c[i] > 448.f ? 448.f : c[i] < -448.f ? -448.f : c[i];
+  }
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
   int hi = __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], 0, false);

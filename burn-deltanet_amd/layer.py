@@ -354,7 +354,9 @@ def quantize_rows(t: Tensor) -> Rows8:
         raise DeltaError(-2, f"quantize_rows: expected [rows, dim], got {list(t.shape)}")
     t = t.float()
     scale = t.abs().amax(1) / 448.0
-    return Rows8(_padded(torch.where(scale[:, None] > 0, t / scale[:, None], t).to(F8)), scale)
+    # A denormal scale may stand for less than a 448th of its row's largest value.
+    codes = torch.where(scale[:, None] > 0, t / scale[:, None], t).clamp(-448.0, 448.0)
+    return Rows8(_padded(codes.to(F8)), scale)
 
 
 def _padded(codes: Tensor) -> Tensor:

@@ -192,3 +192,15 @@ def test_norm_8bit_pads_non_finite_rows_with_zeros_too(dim, bad):
     codes = dn.add_rms_norm_8bit(x, None, torch.ones(dim, device=DEV))[0].codes
     pad = (dim + 15) // 16 * 16
     assert not codes.as_strided((3, pad), (pad, 1)).view(torch.uint8)[:, dim:].any()
+
+
+def test_norm_8bit_of_the_smallest_values_is_finite():
+    """A row whose scale is the smallest number of fp32, and stands for 1.4 of it."""
+    announce("add_rms_norm_8bit: rows of denormal values")
+    tiny = 2.0 ** -149
+    w = (torch.arange(0, 628, device=DEV, dtype=torch.float64) * tiny).float()
+    q, _ = dn.add_rms_norm_8bit(torch.ones(2, 628, device=DEV), None, w)
+    assert (q.scale.double() == tiny).all()
+    codes = q.codes.float()
+    assert torch.isfinite(codes).all()
+    assert (codes[:, 448:] == 448).all() and (codes[:, :16].cpu() == torch.arange(16.)).all()
