@@ -4,7 +4,8 @@ and the gated feed-forward block, each with its gradients.
 
 The reference's blocks end at their projections; these are what a layer built
 on them needs next. `add_rms_norm`, `linear` and `gated_ffn` take part in
-torch's autograd where an input requires a gradient; the `*_forward` and
+torch's autograd where an input requires a gradient (of first order: a second
+derivative is refused); the `*_forward` and
 `*_backward` functions are the two halves for programs that run their own
 backward pass. Weights lie as Burn's Linear holds them, [in, out], applied as
 x @ weight. Every computation is a call into libdeltanet_core.so.
@@ -21,6 +22,7 @@ from torch import Tensor
 
 from . import abi
 from .abi import DeltaError
+from .autograd import first_order
 
 
 class Activation(IntEnum):
@@ -199,6 +201,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return out, (total if residual is not None else total.view_as(total))
 
     @staticmethod
+    @first_order
     def backward(ctx, d_out, d_sum):
         total, weight = ctx.saved_tensors
         if d_out is None:
@@ -292,6 +295,7 @@ class _Linear(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, d_out):
         x, weight, preact = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -462,6 +466,7 @@ class _GatedFfn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, d_out):
         x, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
         need = ctx.needs_input_grad

@@ -204,3 +204,39 @@ def test_norm_8bit_of_the_smallest_values_is_finite():
     codes = q.codes.float()
     assert torch.isfinite(codes).all()
     assert (codes[:, 448:] == 448).all() and (codes[:, :16].cpu() == torch.arange(16.)).all()
+
+
+# -- differentiation ---------------------------------------------------------------
+
+
+def operators(g, T=F32, lead=(2, 3), res=(2, 3)):
+    """(name, operator, its inputs): each differentiable operator as a function of
+    all its inputs."""
+    x = normal(g, *lead, 24, dtype=T)
+    r24, r40 = normal(g, *res, 24, dtype=T), normal(g, *res, 40, dtype=T)
+    w, b = normal(g, 24, 40, dtype=T, scale=0.2), normal(g, 40, dtype=T)
+    wg, wu = normal(g, 24, 56, dtype=T, scale=0.2), normal(g, 24, 56, dtype=T, scale=0.2)
+    wd = normal(g, 56, 24, dtype=T, scale=0.2)
+    return [
+        ("add_rms_norm", lambda x, r, w: dn.add_rms_norm(x, r, w)[0], (x, r24, normal(g, 24, dtype=T))),
+        ("linear", lambda x, w, b, r: dn.linear(x, w, b, dn.Activation.SILU, r), (x, w, b, r40)),
+        ("gated_ffn", lambda x, g, u, d, r: dn.gated_ffn(x, g, u, d, residual=r),
+         (x, wg, wu, wd, r24)),
+    ]
+
+
+@pytest.mark.parametrize("which", range(3), ids=["add_rms_norm", "linear", "gated_ffn"])
+@pytest.mark.parametrize("cotangent", ["of the output", "constant"])
+def test_second_derivatives_are_refused(which, cotangent):
+    """A penalty on the gradient would otherwise lose its part without a word."""
+    name, fn, leaves = operators(gen(31))[which]
+    announce(f"{name}: gradient of a gradient, cotangent {cotangent}")
+    leaves = [t.requires_grad_(True) for t in leaves]
+    out = fn(*leaves)
+    loss = out.sum() if cotangent == "constant" else out.square().sum()
+    plain = torch.autograd.grad(loss, leaves, retain_graph=True)
+    graphed = torch.autograd.grad(loss, leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graphed))
+    with pytest.raises(dn.DeltaError, match="second derivative") as e:
+        (loss + graphed[0].square().sum()).backward()
+    assert e.value.code == -9
