@@ -29,10 +29,10 @@ def first_order(backward):
 
     @functools.wraps(backward)
     def wrapped(ctx, *cotangents):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *cotangents)
         with torch.no_grad():
             grads = backward(ctx, *cotangents)
-        if not torch.is_grad_enabled():
-            return grads
         there = [t for t in grads if t is not None]
         last = iter(_Last.apply(*(t.detach().requires_grad_(True) for t in there)) if there else ())
         return tuple(None if t is None else next(last) for t in grads)

@@ -18,6 +18,7 @@ import torch
 
 from . import abi
 from .abi import DeltaError
+from .autograd import first_order
 
 Tensor = torch.Tensor
 
@@ -319,7 +320,8 @@ def combined_backward(d_y_bshv, d_final_state_bhkv, q_bshk, k_bshk, v_bshv, eras
 
 class DeltaChunkFunction(torch.autograd.Function):
     """The custom autodiff node of chunk_recalculated/backward.rs:31-265: keeps
-    only the seven leaves and runs combined_backward on the way back."""
+    only the seven leaves and runs combined_backward on the way back; a second
+    derivative is refused."""
 
     @staticmethod
     def forward(ctx, q, k, v, erase, write, g, state, chunk_len, scale, check_finite):
@@ -333,6 +335,7 @@ class DeltaChunkFunction(torch.autograd.Function):
         return y, s_out
 
     @staticmethod
+    @first_order
     def backward(ctx, d_y, d_state):
         q, k, v, erase, write, g, state = ctx.saved_tensors
         if d_y is None:

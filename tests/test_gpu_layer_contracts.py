@@ -240,3 +240,19 @@ def test_second_derivatives_are_refused(which, cotangent):
     with pytest.raises(dn.DeltaError, match="second derivative") as e:
         (loss + graphed[0].square().sum()).backward()
     assert e.value.code == -9
+
+
+@pytest.mark.parametrize("cotangent", ["of the output", "constant"])
+def test_second_derivatives_of_the_delta_rule_are_refused(cotangent):
+    announce(f"DeltaInput.run: gradient of a gradient, cotangent {cotangent}")
+    g = gen(32)
+    q, k, v = (normal(g, 1, 64, 2, 64, scale=0.1).requires_grad_(True) for _ in range(3))
+    gates = torch.rand(1, 64, 2, 1, generator=g, device=DEV)
+    y, _ = dn.DeltaInput(q, k, v, gates, gates, None, torch.zeros(1, 2, 64, 64, device=DEV)).run()
+    loss = y.sum() if cotangent == "constant" else y.square().sum()
+    plain = torch.autograd.grad(loss, (q, k, v), retain_graph=True)
+    graphed = torch.autograd.grad(loss, (q, k, v), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graphed))
+    with pytest.raises(dn.DeltaError, match="second derivative") as e:
+        (loss + graphed[0].square().sum()).backward()
+    assert e.value.code == -9
