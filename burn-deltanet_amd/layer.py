@@ -4,8 +4,8 @@ and the gated feed-forward block, each with its gradients.
 
 The reference's blocks end at their projections; these are what a layer built
 on them needs next. `add_rms_norm`, `linear` and `gated_ffn` take part in
-torch's autograd where an input requires a gradient (of first order: a second
-derivative is refused); the `*_forward` and
+torch's autograd where an input requires a gradient, of first order: second
+derivatives and forward-mode tangents are refused. The `*_forward` and
 `*_backward` functions are the two halves for programs that run their own
 backward pass. Weights lie as Burn's Linear holds them, [in, out], applied as
 x @ weight. Every computation is a call into libdeltanet_core.so.
@@ -19,6 +19,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import abi
 from .abi import DeltaError
@@ -126,9 +127,15 @@ def _x_shape(x: Tensor) -> Tuple[int, int]:
 
 
 def _grows(*ts) -> bool:
+    """Whether a derivative is wanted: one of the backward pass, or (it is
+    refused there, as the function has none) a tangent of the forward one."""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False
 

@@ -256,3 +256,19 @@ def test_second_derivatives_of_the_delta_rule_are_refused(cotangent):
     with pytest.raises(dn.DeltaError, match="second derivative") as e:
         (loss + graphed[0].square().sum()).backward()
     assert e.value.code == -9
+
+
+@pytest.mark.parametrize("which", range(3), ids=["add_rms_norm", "linear", "gated_ffn"])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_tangents_are_refused(which, grad_mode):
+    name, fn, leaves = operators(gen(33))[which]
+    announce(f"{name}: forward-mode differentiation, grad mode {grad_mode}")
+    ad = torch.autograd.forward_ad
+    with ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        want = fn(*leaves)  # no tangents: as ever
+        for i in range(len(leaves)):
+            dual = list(leaves)
+            dual[i] = ad.make_dual(leaves[i], torch.ones_like(leaves[i]))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                fn(*dual)
+    assert torch.equal(fn(*leaves), want)
