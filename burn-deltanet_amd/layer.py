@@ -140,6 +140,11 @@ def _grows(*ts) -> bool:
     return False
 
 
+def _shaped(grad: Tensor, shape) -> Optional[Tensor]:
+    """A residual's gradient: its leading axes may be others than the output's."""
+    return None if shape is None else grad.reshape(shape)
+
+
 def _p(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -202,7 +207,7 @@ class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         out, _, total = _norm(x, residual, weight, eps, False)
-        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.eps, ctx.residual_shape = eps, None if residual is None else residual.shape
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(total, weight)
         return out, (total if residual is not None else total.view_as(total))
@@ -212,10 +217,10 @@ class _AddRmsNorm(torch.autograd.Function):
     def backward(ctx, d_out, d_sum):
         total, weight = ctx.saved_tensors
         if d_out is None:
-            return d_sum, d_sum if ctx.has_residual else None, None, None
+            return d_sum, _shaped(d_sum, ctx.residual_shape), None, None
         d_x, d_w = add_rms_norm_backward(d_out, d_sum, total, weight, ctx.eps,
                                          need_weight=ctx.needs_input_grad[2])
-        return d_x, d_x if ctx.has_residual else None, d_w, None
+        return d_x, _shaped(d_x, ctx.residual_shape), d_w, None
 
 
 def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor,
@@ -297,7 +302,8 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         out, preact = _linear(x, weight, bias, activation, residual, True)
-        ctx.activation, ctx.has_bias = activation, bias is not None
+        ctx.activation = activation
+        ctx.residual_shape = None if residual is None else residual.shape
         ctx.save_for_backward(x, weight, preact)
         return out
 
@@ -308,7 +314,8 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         g = linear_backward(d_out, x, weight, preact, ctx.activation, bias=need[2], need_x=need[0],
                             need_weight=need[1])
-        return g.d_x, g.d_weight, g.d_bias, d_out if need[3] else None, None
+        return (g.d_x, g.d_weight, g.d_bias,
+                _shaped(d_out, ctx.residual_shape) if need[3] else None, None)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
@@ -469,6 +476,7 @@ class _GatedFfn(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, w_down, residual, activation):
         out, gate, up = _ffn(x, w_gate, w_up, w_down, activation, residual, True)
         ctx.activation = activation
+        ctx.residual_shape = None if residual is None else residual.shape
         ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
         return out
 
@@ -480,7 +488,7 @@ class _GatedFfn(torch.autograd.Function):
         g = gated_ffn_backward(d_out, x, w_gate, w_up, w_down, gate, up, ctx.activation,
                                need_x=need[0], need_in=need[1] or need[2], need_down=need[3])
         return (g.d_x, g.d_w_gate if need[1] else None, g.d_w_up if need[2] else None, g.d_w_down,
-                d_out if need[4] else None, None)
+                _shaped(d_out, ctx.residual_shape) if need[4] else None, None)
 
 
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,

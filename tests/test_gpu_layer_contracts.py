@@ -272,3 +272,29 @@ def test_tangents_are_refused(which, grad_mode):
             with pytest.raises(NotImplementedError, match="jvp"):
                 fn(*dual)
     assert torch.equal(fn(*leaves), want)
+
+
+@pytest.mark.parametrize("which", range(3), ids=["add_rms_norm", "linear", "gated_ffn"])
+def test_gradient_of_a_residual_has_its_shape(which):
+    name, fn, leaves = operators(gen(34), lead=(2, 3), res=(6,))[which]
+    announce(f"{name}: x [2, 3, dim], residual [6, dim]")
+    at = 1 if name == "add_rms_norm" else -1
+    leaves = [t.requires_grad_(True) for t in leaves]
+    out = fn(*leaves)
+    assert out.shape[:2] == (2, 3)
+    c = normal(gen(35), *out.shape)
+    got = torch.autograd.grad(out, leaves, c)
+    same = list(leaves)
+    same[at] = leaves[at].detach().reshape(2, 3, -1).requires_grad_(True)
+    want = torch.autograd.grad(fn(*same), same, c)
+    for a, b, leaf in zip(got, want, leaves):
+        assert a.shape == leaf.shape and torch.equal(a, b.reshape(a.shape))
+
+
+def test_only_the_sum_of_a_norm_used_with_a_residual_of_another_shape():
+    announce("add_rms_norm: only the sum's gradient, residual [6, dim]")
+    g = gen(36)
+    x, r = normal(g, 2, 3, 24).requires_grad_(True), normal(g, 6, 24).requires_grad_(True)
+    c = normal(g, 2, 3, 24)
+    gx, gr = torch.autograd.grad(dn.add_rms_norm(x, r, normal(g, 24))[1], (x, r), c)
+    assert torch.equal(gx, c) and torch.equal(gr, c.reshape(6, 24))
