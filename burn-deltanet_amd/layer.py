@@ -140,9 +140,9 @@ def _grows(*ts) -> bool:
     return False
 
 
-def _shaped(grad: Tensor, shape) -> Optional[Tensor]:
+def _shaped(grad: Optional[Tensor], shape) -> Optional[Tensor]:
     """A residual's gradient: its leading axes may be others than the output's."""
-    return None if shape is None else grad.reshape(shape)
+    return None if grad is None or shape is None else grad.reshape(shape)
 
 
 def _p(t: Optional[Tensor]):

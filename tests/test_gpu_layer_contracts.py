@@ -298,3 +298,29 @@ def test_only_the_sum_of_a_norm_used_with_a_residual_of_another_shape():
     c = normal(g, 2, 3, 24)
     gx, gr = torch.autograd.grad(dn.add_rms_norm(x, r, normal(g, 24))[1], (x, r), c)
     assert torch.equal(gx, c) and torch.equal(gr, c.reshape(6, 24))
+
+
+def test_autograd_of_the_products_matches_the_explicit_halves():
+    announce("autograd of gated_ffn and of linear's residual")
+    g = gen(37)
+    A = dn.Activation
+    (_, _, (x, w, b, r40)), (_, _, (_, wg, wu, wd, r24)) = operators(g, BF)[1:]
+    for act in (A.SILU, A.GELU):
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd, r24)]
+        y = dn.gated_ffn(*leaves[:4], act, leaves[4])
+        dy = normal(g, *y.shape, dtype=BF)
+        got = torch.autograd.grad(y, leaves, dy)
+        out, gate, up = dn.gated_ffn_forward(x, wg, wu, wd, act, r24)
+        assert torch.equal(out, y)
+        want = dn.gated_ffn_backward(dy, x, wg, wu, wd, gate, up, act)
+        for a, b_ in zip(got, (*want, dy)):
+            assert torch.equal(a, b_)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b, r40)]
+    y = dn.linear(*leaves[:3], A.RELU, leaves[3])
+    dy = normal(g, *y.shape, dtype=BF)
+    got = torch.autograd.grad(y, leaves, dy)
+    out, pre = dn.linear_forward(x, w, b, A.RELU, r40)
+    assert torch.equal(out, y)
+    want = dn.linear_backward(dy, x, w, pre, A.RELU, bias=True)
+    for a, b_ in zip(got, (*want, dy)):
+        assert torch.equal(a, b_)
