@@ -122,8 +122,9 @@ __device__ inline void each(F f) {
   each_of(std::make_integer_sequence<int, N>{}, f);
 }
 
-// act(z) and its derivative. GELU is the exact form, z·Φ(z).
-__device__ inline float gelu_cdf(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
+// act(z) and its derivative. GELU is the exact form, z·Φ(z), with Φ by erfc:
+// 1 + erf(z/√2) loses its bits below zero (4 % at z = −5, all of them at −5.6).
+__device__ inline float gelu_cdf(float z) { return 0.5f * erfcf(z * -0.70710678118654752f); }
 // a[i] = act(z[i]), and with SLOPE d[i] = act'(z[i]): one branch for eight (a
 // may be z).
 template <bool SLOPE>

@@ -324,3 +324,40 @@ def test_autograd_of_the_products_matches_the_explicit_halves():
     want = dn.linear_backward(dy, x, w, pre, A.RELU, bias=True)
     for a, b_ in zip(got, (*want, dy)):
         assert torch.equal(a, b_)
+
+
+# -- GELU's tail ---------------------------------------------------------------------
+
+
+def gelu_points():
+    z = torch.cat([torch.linspace(-12, 6, 1801, device=DEV), torch.linspace(-1, 1, 401, device=DEV)])
+    return z.float().reshape(-1, 1)
+
+
+@pytest.mark.parametrize("rows", [40, 2202])
+def test_gelu_keeps_its_tail(rows):
+    """One term with a weight of one: the argument z is exact. Its scaling by a
+    rounded 1/sqrt(2) is off by 2u, which moves the normal distribution function
+    by at most 2(z^2 + 1)u of itself; erfc is good to 16 ulps (the most that
+    OpenCL allows it), 32u, and a few products follow: (2 z^2 + 40)u."""
+    announce(f"linear {rows}x1x4 fp32 gelu: its tail")
+    z = gelu_points()
+    z = z[:: max(1, z.shape[0] // rows)][:rows].contiguous()
+    got = dn.linear(z, torch.ones(1, 4, device=DEV), None, dn.Activation.GELU)
+    z = z.expand(-1, 4)
+    want = R.act(d(z), "gelu")
+    R.check(got, (want, (2 * d(z) ** 2 + 40) * R.U * want.abs() + 1e-37), "gelu")
+
+
+def test_slope_of_gelu_keeps_its_tail():
+    """Its two terms, each as above (the exponential's argument is off by 2u of
+    z^2/2, and it is good to 2 ulps), add up with their errors."""
+    announce("linear_backward fp32 gelu: its tail")
+    z, one = gelu_points(), torch.ones(1, 1, device=DEV)
+    got = dn.linear_backward(torch.ones_like(z), z, one, z, dn.Activation.GELU,
+                             need_weight=False).d_x
+    zz = d(z)
+    cdf = 0.5 * torch.erfc(-zz / math.sqrt(2.0))
+    rest = zz * torch.exp(-zz * zz / 2) / math.sqrt(2 * math.pi)
+    bound = (2 * zz ** 2 + 40) * R.U * (cdf + rest.abs()) + 1e-37
+    R.check(got, (cdf + rest, bound), "slope")
