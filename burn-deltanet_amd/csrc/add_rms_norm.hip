@@ -109,6 +109,8 @@ __device__ inline void store_codes(uint8_t* row, int end, int col, int dim, uint
 }
 
 constexpr int kNormThreads = 256;
+// Workgroups along x: a launch of 2^32 threads or more along an axis wraps.
+constexpr int kMostGroups = 1 << 20;
 
 // NCH chunks of 8 values a lane; NCH = 0: any length, in two passes.
 template <class T, class TW, bool F8, int WPR, int NCH>
@@ -116,8 +118,9 @@ __global__ __launch_bounds__(kNormThreads) void add_rms_norm_kernel(NormArgs p) 
   constexpr int kLanes = 64 * WPR;  // lanes to a row
   __shared__ float red[2][4];
   const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t row = WPR == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (row >= p.rows) return;  // whole waves; with WPR = 4 there is no such row
+  const int64_t group = int64_t(blockIdx.y) * kMostGroups + blockIdx.x;
+  const int64_t row = WPR == 1 ? group * 4 + (threadIdx.x >> 6) : group;
+  if (row >= p.rows) return;  // whole waves; with WPR = 4 whole workgroups
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
   const TW* weight = static_cast<const TW*>(p.weight);
@@ -418,7 +421,10 @@ Shape shape_of(int64_t rows, int64_t dim) {
 template <class T, class TW, bool F8>
 hipError_t fwd_go(const NormArgs& p, hipStream_t stream) {
   const Shape s = shape_of(p.rows, p.dim);
-  const dim3 grid(unsigned(s.wpr == 1 ? (p.rows + 3) / 4 : p.rows)), block(kNormThreads);
+  const int64_t groups = s.wpr == 1 ? (int64_t(p.rows) + 3) / 4 : p.rows;
+  const dim3 grid(unsigned(std::min<int64_t>(groups, kMostGroups)),
+                  unsigned((groups + kMostGroups - 1) / kMostGroups)),
+      block(kNormThreads);
   if (s.wpr == 1 && s.nch == 1)
     hipLaunchKernelGGL((add_rms_norm_kernel<T, TW, F8, 1, 1>), grid, block, 0, stream, p);
   else if (s.wpr == 1 && s.nch == 2)

@@ -361,3 +361,23 @@ def test_slope_of_gelu_keeps_its_tail():
     rest = zz * torch.exp(-zz * zz / 2) / math.sqrt(2 * math.pi)
     bound = (2 * zz ** 2 + 40) * R.U * (cdf + rest.abs()) + 1e-37
     R.check(got, (cdf + rest, bound), "slope")
+
+
+# -- sizes ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_norm_of_more_rows_than_a_launch_has_threads_for(eight_bit):
+    rows = (1 << 26) + 5
+    announce(f"add_rms_norm {rows}x1, 8-bit {eight_bit}")
+    x, w = normal(gen(40), rows, 1, dtype=BF), torch.full((1,), 1.5, dtype=BF, device=DEV)
+    if eight_bit:
+        (codes, scale), _ = dn.add_rms_norm_8bit(x, None, w)
+        top = 1.5 * (x.float() / (x.float().square() + 1e-5).sqrt()).abs()[:, 0]
+        assert ((scale * 448 - top).abs() <= 1e-5 * top).all()
+        sign = torch.where(x[:, 0] < 0, -448.0, 448.0)
+        assert ((codes[:, 0].float() == sign) | (scale == 0)).all()
+    else:
+        out, _ = dn.add_rms_norm(x, None, w)
+        for part in (slice(0, 1000), slice((1 << 26) - 1000, rows)):
+            R.check(out[part], R.norm(d(x[part]), None, d(w), 1e-5, BF)[1], "out")
