@@ -296,7 +296,8 @@ Plan plan_product(const GemmArgs& g, GemmForm form, GemmEpi epi, int dtype) {
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
       const int64_t per = ceil_div(ksteps, s);
       const int split = int(ceil_div(ksteps, per));
-      if (tiles * split > (int64_t(1) << 30)) break;
+      // A launch of 2^32 threads or more wraps.
+      if (tiles * split >= (int64_t(1) << 32) / (tile == kTileLone ? 512 : 256)) break;
       const int64_t w = ceil_div(tiles * split, cus), left = w % t.most;
       const auto turn = [&](int64_t n) {
         return double(per) * std::max(t.lone, t.each * double(n)) + t.ends;
@@ -355,6 +356,7 @@ hipError_t join_typed(const GemmArgs& g, GemmEpi epi, GemmTile tile, hipStream_t
 
 hipError_t run_product(GemmArgs& g, GemmForm form, GemmEpi epi, int dtype, int out_dtype,
                        const Plan& plan, float* partial, const char* name, hipStream_t stream) {
+  if (!plan.split) return hipErrorInvalidConfiguration;  // no tile is large enough
   apply(g, plan, epi == kEpiGated, partial);
   hipError_t e;
   {

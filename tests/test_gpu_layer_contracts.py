@@ -381,3 +381,14 @@ def test_norm_of_more_rows_than_a_launch_has_threads_for(eight_bit):
         out, _ = dn.add_rms_norm(x, None, w)
         for part in (slice(0, 1000), slice((1 << 26) - 1000, rows)):
             R.check(out[part], R.norm(d(x[part]), None, d(w), 1e-5, BF)[1], "out")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_of_more_rows_than_a_launch_has_threads_for(dtype):
+    rows, T = (1 << 30) + 77, TYPES[dtype]
+    announce(f"linear {rows}x1x1 {dtype}")
+    x = torch.empty(rows, 1, dtype=T, device=DEV)
+    x[:, 0] = torch.arange(rows, device=DEV, dtype=torch.int32).remainder_(251).to(T)
+    w = torch.full((1, 1), 3.0, dtype=T, device=DEV)
+    out = dn.linear(x, w)
+    assert torch.equal(out, x * w)
