@@ -319,30 +319,53 @@ __device__ inline void finish8(const GemmArgs& p, int z, int sp, int64_t row, in
 }
 
 // One HBM → LDS copy of 16 bytes a lane: lane i's word goes to `lds` + 16·i.
-// No register receives it; it is complete when vmcnt says so. Nothing else in
-// these kernels uses m0 (LDS accesses do not need it on this architecture).
+// No register receives it; it is complete when vmcnt says so. The compiler does
+// not look inside the text, so it holds the wait that the copy owes m0. Nothing
+// else in these kernels uses m0 (LDS accesses do not need it on this architecture).
 __device__ inline void copy_to_lds(const char* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(src)
                : "memory");
 }
+// The same from a scalar base. A vector instruction may have written it just
+// before, which a copy may read five wait states later, the scalar unit at once:
+// that unit's copy of it also is m0's wait (with five states in its place the
+// wide kernel takes 2 to 4 % longer).
+__device__ inline void copy_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+  const char* from;
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+               : "=&s"(from)
+               : "s"(lds), "v"(offset), "s"(base)
+               : "memory");
+}
 // c += b·a with c held in accumulation registers. The wide kernel's 256 sums
 // fill that half of the register file; left to itself the compiler moves them
-// between the halves at every branch (276 moves a k tile of 128 products, and
-// spills). It does not see a matrix instruction here: settle_acc() is owed
-// before anything else reads the sums.
+// between the halves at every branch (276 moves a k tile of 128 products). What
+// it spills with them there are addresses, outside the products. It does not see
+// a matrix instruction here: settle_acc() is owed before anything else reads the
+// sums, and settle_words() before operands that a vector instruction wrote.
 __device__ inline void mfma16_acc(const uint4& b, const uint4& a, f32x4& c) {
   asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
       : "+a"(c)
       : "v"(__builtin_bit_cast(bf16x8, b)), "v"(__builtin_bit_cast(bf16x8, a)));
 }
 // The wait that a matrix instruction's result needs before another kind of
-// instruction reads it, tied to eight of the sums.
+// instruction reads it, by itself and tied to eight of the sums.
+__device__ inline void settle_products() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 __device__ inline void settle_acc(f32x4 (&c)[8]) {
   asm volatile("s_nop 15\n\ts_nop 15"
                : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]),
                  "+a"(c[6]), "+a"(c[7]));
+}
+
+// The wait that a vector instruction's result needs before a matrix instruction
+// reads it, tied to widened codes. (In the products' own text the two states
+// would cost the wide kernel 6 %.)
+__device__ inline void settle_words(Codes16& c) {
+  bf16x8 lo = __builtin_bit_cast(bf16x8, c.lo), hi = __builtin_bit_cast(bf16x8, c.hi);
+  asm("s_nop 1" : "+v"(lo), "+v"(hi));
+  c = {__builtin_bit_cast(uint4, lo), __builtin_bit_cast(uint4, hi)};
 }
 
 template <int N>
@@ -920,10 +943,7 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
   };
   const uint32_t lds0 = lds_address(smem) + uint32_t(wave) * 1024;
   auto copy = [&](uint32_t at, uint32_t offset, const char* base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds0 + at), "v"(offset), "s"(base)
-                 : "memory");
+    copy_to_lds(base, offset, lds0 + at);
   };
   // Buffers: A's of tile t is (t − t0) % 3, B's (t − t0) % 2.
   auto copy_a = [&](int buf, int w) { copy(uint32_t(buf * kHalf + w * 4096), oa[w], ba); };
@@ -1035,8 +1055,12 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
         if constexpr (kF8) {
           if constexpr (i == 0)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) wb[j] = widen(fb[kk][j]);
+            for (int j = 0; j < 8; ++j) {
+              wb[j] = widen(fb[kk][j]);
+              settle_words(wb[j]);
+            }
           a = widen(fa[kk][i]);
+          settle_words(a);
         }
         each<8>([&](auto jn) {
           constexpr int j = decltype(jn)::value;
@@ -1075,6 +1099,9 @@ __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
       each<8>([&](auto n) { work(std::integral_constant<int, 8 + n.value>{}); });
       advance();
       abuf = anext;
+      // Where the loop ends the compiler may move sums already (it did so 14 states
+      // after the last product).
+      if (t + 1 == t1) settle_products();
     }
   }
   __syncthreads();
