@@ -416,10 +416,10 @@ __device__ inline void tile_word(int L, int& r, int& c) {
 // 16-byte steps go through registers, with masks.
 //
 // Bound by LDS and the copies, 50 to 60 GB/s a CU, at two workgroups a CU 0.58 us
-// a k tile of 128 x 128. Measured, bf16 x·W: 4096 x 4096 x 2048 75 us (910
-// TFLOP/s), 1500 x 2048 x 12304 99 (760), 1024 x 2048 x 5632 38 (620); 8-bit
-// 4096 x 4096 x 2048 65 (1050). fp32 is bound by the matrix unit: 2048 x 1024 x
-// 2048 76 us (113 TFLOP/s); 500 x 256 x 1039 with unaligned rows 16, all latency.
+// a k tile of 128 x 128. Measured, bf16 x·W: 4096 x 4096 x 2048 70 us (980
+// TFLOP/s), 1500 x 2048 x 12304 95 (800), 1024 x 2048 x 5632 36 (650); 8-bit
+// 4096 x 4096 x 2048 62 (1100). fp32 is bound by the matrix unit: 2048 x 2048 x
+// 1024 77 us (111 TFLOP/s); 500 x 256 x 1039 with unaligned rows 16, all latency.
 template <class T, class TO, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, int WK,
           int RING, int EPI, bool STAGED>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) {
@@ -816,10 +816,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void gemm_kernel(GemmArgs p) 
 //
 // Bound by the matrix unit's clock and by what of the loop does not hide behind
 // it: a k tile takes 1.65 us on all CUs (1.3 PFLOP/s), a round of tiles 5 to 9 us
-// of ends. Measured, bf16: 16384 x 4096 x 2048 x·W 260 us (1057 TFLOP/s), its
-// gradients 465 together; 8192 x 2048 x 12304 400 (1032); the feed-forward of
-// 16384 x 2048 x 5632 925, its backward 2157. 8-bit: 3.2 us a k tile of 128, the
-// bf16 rate.
+// of ends. Measured, bf16: 16384 x 4096 x 2048 x·W 217 us (1270 TFLOP/s), with a
+// residual 239, its gradients 485 together; 8192 x 2048 x 12304 400 (1030); the
+// feed-forward of 16384 x 2048 x 5632 942, its backward 2170. 8-bit: 3.2 us a k
+// tile of 128, the bf16 rate; 8192 x 4096 x 4096 282 us (975).
 template <class T, class TO, bool ACOL, bool BCOL, int EPI>
 __global__ __launch_bounds__(256, 1) void gemm_wide_kernel(GemmArgs p) {
   using namespace gemm;

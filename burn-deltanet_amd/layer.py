@@ -8,7 +8,8 @@ torch's autograd where an input requires a gradient, of first order: second
 derivatives and forward-mode tangents are refused. The `*_forward` and
 `*_backward` functions are the two halves for programs that run their own
 backward pass. Weights lie as Burn's Linear holds them, [in, out], applied as
-x @ weight. Every computation is a call into libdeltanet_core.so.
+x @ weight. Every computation is a call into libdeltanet_core.so, but for
+quantize_rows, which lays weights out once.
 """
 
 from __future__ import annotations
@@ -321,7 +322,9 @@ class _Linear(torch.autograd.Function):
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
            activation: Activation = Activation.IDENTITY,
            residual: Optional[Tensor] = None) -> Tensor:
-    """act(x @ weight + bias) + residual, weight [in, out]."""
+    """act(x @ weight + bias) + residual, weight [in, out]. An operand whose last
+    axis is not contiguous, such as the transposed view of a weight [out, in], is
+    copied in every call: a program lays such a weight out once."""
     if _grows(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
     return _linear(x, weight, bias, activation, residual, False)[0]
@@ -406,8 +409,9 @@ def linear_8bit(x: Rows8, weight: Rows8, bias: Optional[Tensor] = None,
                 activation: Activation = Activation.IDENTITY, residual: Optional[Tensor] = None,
                 out_dtype=torch.bfloat16) -> Tensor:
     """act(x @ weightᵀ + bias) + residual from operands in 8 bits: x [rows, in]
-    and weight [out, in], as add_rms_norm_8bit and quantize_rows make them.
-    bias, residual and the output are of `out_dtype`. No gradient."""
+    and weight [out, in], as add_rms_norm_8bit and quantize_rows make them, or
+    columns of such from a multiple of 16 on (other views are copied in every
+    call). bias, residual and the output are of `out_dtype`. No gradient."""
     c, w = _codes(x, "x"), _codes(weight, "weight")
     rows, k = c.shape
     n = w.shape[0]

@@ -415,8 +415,10 @@ int dn_block_step(const dn_block_step_args *args, hipStream_t stream);
  * the element's own). rows may be 0: the forwards then do nothing, and the
  * backwards write zeros to the weights' gradients. Widths are at most 2^24, and
  * every tensor is below 2^40 elements. Sums, norms and products accumulate in
- * fp32. No output may alias an input except where said; workspaces as for the
- * chunk calls (dn_*_workspace_bytes, 16-byte aligned, NULL: the library's). */
+ * fp32. No output may alias an input except where said (then with the input's
+ * stride); workspaces as for the chunk calls (dn_*_workspace_bytes, 16-byte
+ * aligned, NULL: the library's). A size depends on the tensors' alignment too, so
+ * it is asked for with the call's own arguments. */
 
 /* sum = x + residual; out = sum / sqrt(mean(sum^2) + eps) * weight, per row of
  * `dim` values, from the unrounded sum. With out_dtype DN_F8: scale[row] =
