@@ -341,10 +341,11 @@ __device__ inline void copy_to_lds(const char* base, uint32_t offset, uint32_t l
 }
 // c += b·a with c held in accumulation registers. The wide kernel's 256 sums
 // fill that half of the register file; left to itself the compiler moves them
-// between the halves at every branch (276 moves a k tile of 128 products). What
-// it spills with them there are addresses, outside the products. It does not see
-// a matrix instruction here: settle_acc() is owed before anything else reads the
-// sums, and settle_words() before operands that a vector instruction wrote.
+// between the halves at every branch (276 moves a k tile of 128 products, and
+// spills among them). What scratch memory the kernel uses now lies outside the
+// products. The compiler does not see a matrix instruction here: settle_acc() is
+// owed before anything else reads the sums, and settle_words() before a product
+// reads operands that a vector instruction wrote.
 __device__ inline void mfma16_acc(const uint4& b, const uint4& a, f32x4& c) {
   asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
       : "+a"(c)
