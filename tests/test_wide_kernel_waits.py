@@ -141,7 +141,7 @@ def faults(code):
 
 
 def listed(*lines):
-    """Instructions at consecutive addresses, for the checker's own tests."""
+    """Instructions at consecutive addresses, for tests of the reading itself."""
     return [Instruction(f"{line} // {4 * n:012X}: 00000000") for n, line in enumerate(lines)]
 
 
@@ -165,12 +165,12 @@ def listed(*lines):
     (["s_mov_b32 m0, s9", "global_load_lds_dwordx4 v2, s[6:7]"], "m0"),
     (["v_readlane_b32 s4, v9, 3", "global_store_dword v2, v3, s[4:5]"], "address"),
 ])
-def test_the_checker_sees_a_missing_wait(lines, bad):
+def test_a_missing_wait_is_seen(lines, bad):
     found = faults(listed(*lines))
     assert [f.split(":")[0] for f in found] == ([bad] if bad else [])
 
 
-def test_the_checker_follows_a_loop():
+def test_loops_are_followed():
     code = listed("v_mfma_f32_16x16x32_bf16 a[0:3], v[0:3], v[4:7], a[0:3]", "s_nop 0",
                   "v_mov_b32_e32 v4, v9", "s_cbranch_scc1 4")
     assert not faults(code)
