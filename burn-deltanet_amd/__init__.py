@@ -8,7 +8,9 @@ combined_backward, unit_lower_inverse), `frontend` its projection front-end
 (QkvProjection), output norm (OutNorm) and the fused decode step of a block
 (block_step), and `layer` the operators that a decoder layer needs around them:
 the norm with the residual's addition, linear projections (also from 8-bit
-operands) and the gated feed-forward block.
+operands) and the gated feed-forward block. `softmax_attention` is that of
+the layers between delta-rule layers, `stack` the embedding of token ids and the
+joint of a block and the residual stream.
 """
 
 from . import abi
@@ -22,6 +24,10 @@ from .layer import (Activation, GatedFfnGrads, LinearGrads, Rows8, add_rms_norm,
                     add_rms_norm_8bit, add_rms_norm_backward, gated_ffn, gated_ffn_backward,
                     gated_ffn_forward, linear, linear_8bit, linear_backward, linear_forward,
                     quantize_rows)
+from .softmax_attention import (AttentionGrads, KeySpans, attention, attention_backward,
+                                attention_forward)
+from .stack import (BlockNormGrads, block_norm, block_norm_backward, embedding,
+                    embedding_backward)
 
 __all__ = [
     "abi", "DeltaError", "DeltaChunkFunction", "DeltaChunkGrads", "DeltaInput", "DeltaPath",
@@ -32,4 +38,6 @@ __all__ = [
     "Activation", "GatedFfnGrads", "LinearGrads", "Rows8", "add_rms_norm", "add_rms_norm_8bit",
     "add_rms_norm_backward", "gated_ffn", "gated_ffn_backward", "gated_ffn_forward", "linear",
     "linear_8bit", "linear_backward", "linear_forward", "quantize_rows",
+    "AttentionGrads", "KeySpans", "attention", "attention_backward", "attention_forward",
+    "BlockNormGrads", "block_norm", "block_norm_backward", "embedding", "embedding_backward",
 ]

@@ -21,6 +21,7 @@ DN_F32, DN_BF16, DN_F8 = 0, 1, 2
 DN_ALGO_AUTO, DN_ALGO_GENERIC, DN_ALGO_MFMA, DN_ALGO_MFMA_FUSED = 0, 1, 2, 3
 RECURRENT_MAX_K = 512  # dn_recurrent's head_k_dim limit (deltanet_core.h)
 DN_ACT_IDENTITY, DN_ACT_SILU, DN_ACT_RELU, DN_ACT_ELU_PLUS_ONE, DN_ACT_GELU = 0, 1, 2, 3, 4
+DN_GATE_NONE, DN_GATE_CHANNEL, DN_GATE_TOKEN, DN_GATE_FULL = 0, 1, 2, 3
 DN_QKNORM_NONE, DN_QKNORM_L2, DN_QKNORM_SUM = 0, 1, 2
 DN_WRITE_FIXED, DN_WRITE_SCALAR, DN_WRITE_CHANNEL = 0, 1, 2
 FRONTEND_MAX_HEAD_DIM, FRONTEND_MAX_KERNEL = 256, 8
@@ -55,6 +56,10 @@ EXPORTS = [
     "dn_linear", "dn_linear_workspace_bytes", "dn_linear_bwd", "dn_linear_bwd_workspace_bytes",
     "dn_gated_ffn", "dn_gated_ffn_workspace_bytes", "dn_gated_ffn_bwd",
     "dn_gated_ffn_bwd_workspace_bytes",
+    "dn_block_norm", "dn_block_norm_bwd", "dn_block_norm_bwd_workspace_bytes",
+    "dn_embedding", "dn_embedding_bwd", "dn_embedding_bwd_workspace_bytes",
+    "dn_attention", "dn_attention_workspace_bytes", "dn_attention_bwd",
+    "dn_attention_bwd_workspace_bytes",
 ]
 NOALLOC_SCRATCH_BYTES = 64 << 20  # DN_NOALLOC_SCRATCH_BYTES (deltanet_core.h)
 
@@ -222,12 +227,76 @@ class GatedFfnBwdArgs(ctypes.Structure):
     ]
 
 
+class BlockNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("x_stride", _i64), ("residual_stride", _i64),
+        ("gate_stride", _i64), ("sum_stride", _i64), ("out_stride", _i64), ("eps", _f64),
+        ("residual_scale", _f64), ("dtype", _i32), ("weight_dtype", _i32), ("gate_kind", _i32),
+        ("x", _vp), ("residual", _vp), ("pre_weight", _vp), ("post_weight", _vp), ("gate", _vp),
+        ("sum", _vp), ("out", _vp),
+    ]
+
+
+class BlockNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("x_stride", _i64), ("sum_stride", _i64),
+        ("gate_stride", _i64), ("d_out_stride", _i64), ("d_sum_stride", _i64),
+        ("d_x_stride", _i64), ("d_residual_stride", _i64), ("d_gate_stride", _i64), ("eps", _f64),
+        ("residual_scale", _f64), ("dtype", _i32), ("weight_dtype", _i32), ("gate_kind", _i32),
+        ("x", _vp), ("sum", _vp), ("pre_weight", _vp), ("post_weight", _vp), ("gate", _vp),
+        ("d_out", _vp), ("d_sum", _vp), ("d_x", _vp), ("d_residual", _vp), ("d_pre_weight", _vp),
+        ("d_post_weight", _vp), ("d_gate", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("vocab", _i64), ("dim", _i64), ("table_stride", _i64),
+        ("out_stride", _i64), ("scale", _f64), ("dtype", _i32), ("wide_ids", _i32), ("ids", _vp),
+        ("table", _vp), ("out", _vp),
+    ]
+
+
+class EmbeddingBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("vocab", _i64), ("dim", _i64), ("d_out_stride", _i64),
+        ("d_table_stride", _i64), ("scale", _f64), ("dtype", _i32), ("wide_ids", _i32),
+        ("ids", _vp), ("d_out", _vp), ("d_table", _vp), ("workspace", _vp),
+        ("workspace_bytes", _sz),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("key_rows", _i64), ("sequences", _i64), ("nheads", _i64),
+        ("kv_heads", _i64), ("head_dim", _i64), ("q_stride", _i64), ("k_stride", _i64),
+        ("v_stride", _i64), ("out_stride", _i64), ("scale", _f64), ("dtype", _i32),
+        ("causal", _i32), ("q", _vp), ("k", _vp), ("v", _vp), ("offsets", _vp),
+        ("key_starts", _vp), ("key_lengths", _vp), ("out", _vp), ("lse", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class AttentionBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("sequences", _i64), ("nheads", _i64), ("kv_heads", _i64),
+        ("head_dim", _i64), ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64),
+        ("out_stride", _i64), ("d_out_stride", _i64), ("d_q_stride", _i64), ("d_k_stride", _i64),
+        ("d_v_stride", _i64), ("scale", _f64), ("dtype", _i32), ("causal", _i32), ("q", _vp),
+        ("k", _vp), ("v", _vp), ("offsets", _vp), ("out", _vp), ("lse", _vp), ("d_out", _vp),
+        ("d_q", _vp), ("d_k", _vp), ("d_v", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
 # The operators around the mixer: (entry, its argument struct, whether a
 # *_workspace_bytes entry goes with it).
 _LAYER = [
     ("dn_add_rms_norm", AddRmsNormArgs, False), ("dn_add_rms_norm_bwd", AddRmsNormBwdArgs, True),
     ("dn_linear", LinearArgs, True), ("dn_linear_bwd", LinearBwdArgs, True),
     ("dn_gated_ffn", GatedFfnArgs, True), ("dn_gated_ffn_bwd", GatedFfnBwdArgs, True),
+    ("dn_block_norm", BlockNormArgs, False), ("dn_block_norm_bwd", BlockNormBwdArgs, True),
+    ("dn_embedding", EmbeddingArgs, False), ("dn_embedding_bwd", EmbeddingBwdArgs, True),
+    ("dn_attention", AttentionArgs, True), ("dn_attention_bwd", AttentionBwdArgs, True),
 ]
 
 _LIB = None

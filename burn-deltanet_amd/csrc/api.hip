@@ -1153,6 +1153,225 @@ int dn_gated_ffn_bwd(const dn_gated_ffn_bwd_args* a, hipStream_t stream) {
   return e == hipSuccess ? DN_OK : hip_fail(e, "dn_gated_ffn_bwd launch");
 }
 
+namespace {
+
+int check_gate(int kind, const void* gate, int64_t rows, int64_t dim, int64_t stride,
+               const char* what) {
+  if (kind < DN_GATE_NONE || kind > DN_GATE_FULL)
+    return fail(DN_ERR_SHAPE, "gate_kind must be one of dn_gate_kind");
+  if (kind == DN_GATE_NONE) return DN_OK;
+  if (kind != DN_GATE_CHANNEL)
+    return check_rows(gate, rows, kind == DN_GATE_FULL ? dim : 1, stride, what);
+  return gate ? DN_OK : fail(DN_ERR_NULL, std::string(what) + " is NULL");
+}
+
+int check_block_norm(const dn_block_norm_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim})) return rc;
+  if (int rc = check_norm_types(a->dtype, a->weight_dtype, a->eps)) return rc;
+  if (!std::isfinite(a->residual_scale))
+    return fail(DN_ERR_SHAPE, "residual_scale must be finite");
+  if (int rc = check_rows(a->x, a->rows, a->dim, a->x_stride, "x")) return rc;
+  if (int rc = check_rows(a->residual, a->rows, a->dim, a->residual_stride, "residual")) return rc;
+  if (int rc = check_gate(a->gate_kind, a->gate, a->rows, a->dim, a->gate_stride, "gate"))
+    return rc;
+  if (int rc = check_rows(a->sum, a->rows, a->dim, a->sum_stride, "sum")) return rc;
+  if (int rc = check_rows(a->out, a->rows, a->dim, a->out_stride, "out")) return rc;
+  return a->pre_weight ? DN_OK : fail(DN_ERR_NULL, "pre_weight is NULL");
+}
+
+int check_block_norm_bwd(const dn_block_norm_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_sizes(a->rows, {a->dim})) return rc;
+  if (int rc = check_norm_types(a->dtype, a->weight_dtype, a->eps)) return rc;
+  if (!std::isfinite(a->residual_scale))
+    return fail(DN_ERR_SHAPE, "residual_scale must be finite");
+  if (int rc = check_rows(a->x, a->rows, a->dim, a->x_stride, "x")) return rc;
+  if (int rc = check_rows(a->sum, a->rows, a->dim, a->sum_stride, "sum")) return rc;
+  if (int rc = check_gate(a->gate_kind, a->gate, a->rows, a->dim, a->gate_stride, "gate"))
+    return rc;
+  if (int rc = check_rows_opt(a->d_out, a->rows, a->dim, a->d_out_stride, "d_out")) return rc;
+  if (int rc = check_rows_opt(a->d_sum, a->rows, a->dim, a->d_sum_stride, "d_sum")) return rc;
+  if (int rc = check_rows_opt(a->d_x, a->rows, a->dim, a->d_x_stride, "d_x")) return rc;
+  if (int rc = check_rows_opt(a->d_residual, a->rows, a->dim, a->d_residual_stride, "d_residual"))
+    return rc;
+  if (a->d_gate) {
+    if (a->gate_kind == DN_GATE_NONE) return fail(DN_ERR_SHAPE, "d_gate without a gate");
+    if (int rc = check_gate(a->gate_kind, a->d_gate, a->rows, a->dim, a->d_gate_stride, "d_gate"))
+      return rc;
+  }
+  if (!a->pre_weight) return fail(DN_ERR_NULL, "pre_weight is NULL");
+  if (a->d_post_weight && !a->post_weight)
+    return fail(DN_ERR_NULL, "d_post_weight without post_weight");
+  return DN_OK;
+}
+
+int check_embedding_sizes(int64_t tokens, int64_t vocab, int64_t dim, int32_t dtype, double scale) {
+  if (tokens < 0) return fail(DN_ERR_SHAPE, "tokens must not be negative");
+  if (int rc = check_sizes(tokens, {vocab, dim})) return rc;
+  if (tokens > (int64_t(1) << 28)) return fail(DN_ERR_SHAPE, "tensor too large");
+  if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  return std::isfinite(scale) ? DN_OK : fail(DN_ERR_SHAPE, "scale must be finite");
+}
+
+int check_embedding(const dn_embedding_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_embedding_sizes(a->tokens, a->vocab, a->dim, a->dtype, a->scale)) return rc;
+  if (!a->ids && a->tokens > 0) return fail(DN_ERR_NULL, "ids is NULL");
+  if (int rc = check_rows(a->table, a->vocab, a->dim, a->table_stride, "table")) return rc;
+  return check_rows(a->out, a->tokens, a->dim, a->out_stride, "out");
+}
+
+int check_embedding_bwd(const dn_embedding_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_embedding_sizes(a->tokens, a->vocab, a->dim, a->dtype, a->scale)) return rc;
+  if (!a->ids && a->tokens > 0) return fail(DN_ERR_NULL, "ids is NULL");
+  if (int rc = check_rows(a->d_out, a->tokens, a->dim, a->d_out_stride, "d_out")) return rc;
+  return check_rows(a->d_table, a->vocab, a->dim, a->d_table_stride, "d_table");
+}
+
+int check_heads(int64_t tokens, int64_t sequences, int64_t nheads, int64_t kv_heads,
+                int64_t head_dim, int32_t dtype, double scale, const void* offsets) {
+  if (tokens < 0 || sequences < 0)
+    return fail(DN_ERR_SHAPE, "tokens and sequences must not be negative");
+  if (kv_heads < 1 || nheads < 1 || nheads % kv_heads)
+    return fail(DN_ERR_SHAPE, "nheads must be a multiple of kv_heads, both at least 1");
+  if (head_dim < 1) return fail(DN_ERR_SHAPE, "head_dim must be at least 1");
+  if (head_dim > 256) return fail(DN_ERR_UNSUPPORTED, "head_dim must be at most 256");
+  if (nheads > 65536 || tokens > INT32_MAX / 2 || sequences > INT32_MAX / 2 ||
+      (tokens + sequences) * nheads > INT32_MAX / 2)
+    return fail(DN_ERR_SHAPE, "tensor too large");
+  // A launch has fewer than 2^32 threads: tiles of 64 rows at the least.
+  if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 24))
+    return fail(DN_ERR_SHAPE, "tensor too large");
+  if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
+  if (!std::isnan(scale) && !(scale > 0.0 && float(scale) > 0.f && std::isfinite(float(scale))))
+    return fail(DN_ERR_SHAPE, "scale must be a positive number");
+  if (!offsets && tokens > 0 && (sequences < 1 || tokens % sequences))
+    return fail(DN_ERR_SHAPE, "without offsets the sequences must have equal lengths");
+  return DN_OK;
+}
+
+int check_attention(const dn_attention_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_heads(a->tokens, a->sequences, a->nheads, a->kv_heads, a->head_dim, a->dtype,
+                           a->scale, a->offsets))
+    return rc;
+  if (!a->key_starts != !a->key_lengths)
+    return fail(DN_ERR_NULL, "key_starts and key_lengths go together");
+  if (a->key_rows < 0 || a->key_rows > INT32_MAX / 2)
+    return fail(DN_ERR_SHAPE, "key_rows out of range");
+  if (!a->key_starts && a->key_rows != a->tokens)
+    return fail(DN_ERR_SHAPE, "without key spans k and v must have the queries' rows");
+  const int64_t qd = a->nheads * a->head_dim, kd = a->kv_heads * a->head_dim;
+  if (int rc = check_rows(a->q, a->tokens, qd, a->q_stride, "q")) return rc;
+  if (int rc = check_rows(a->k, a->key_rows, kd, a->k_stride, "k")) return rc;
+  if (int rc = check_rows(a->v, a->key_rows, kd, a->v_stride, "v")) return rc;
+  return check_rows(a->out, a->tokens, qd, a->out_stride, "out");
+}
+
+int check_attention_bwd(const dn_attention_bwd_args* a) {
+  if (!a) return fail(DN_ERR_NULL, "args is NULL");
+  if (int rc = check_heads(a->tokens, a->sequences, a->nheads, a->kv_heads, a->head_dim, a->dtype,
+                           a->scale, a->offsets))
+    return rc;
+  const int64_t qd = a->nheads * a->head_dim, kd = a->kv_heads * a->head_dim;
+  if (int rc = check_rows(a->q, a->tokens, qd, a->q_stride, "q")) return rc;
+  if (int rc = check_rows(a->k, a->tokens, kd, a->k_stride, "k")) return rc;
+  if (int rc = check_rows(a->v, a->tokens, kd, a->v_stride, "v")) return rc;
+  if (int rc = check_rows(a->out, a->tokens, qd, a->out_stride, "out")) return rc;
+  if (int rc = check_rows(a->d_out, a->tokens, qd, a->d_out_stride, "d_out")) return rc;
+  if (!a->lse && a->tokens > 0) return fail(DN_ERR_NULL, "lse is NULL");
+  if (int rc = check_rows_opt(a->d_q, a->tokens, qd, a->d_q_stride, "d_q")) return rc;
+  if (int rc = check_rows_opt(a->d_k, a->tokens, kd, a->d_k_stride, "d_k")) return rc;
+  return check_rows_opt(a->d_v, a->tokens, kd, a->d_v_stride, "d_v");
+}
+
+float attention_scale(double scale, int64_t head_dim) {
+  return std::isnan(scale) ? float(1.0 / std::sqrt(double(head_dim))) : float(scale);
+}
+
+}  // namespace
+
+int dn_block_norm(const dn_block_norm_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_block_norm(a)) return rc;
+  if (a->rows == 0) return DN_OK;
+  const hipError_t e = launch_block_norm(*a, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_block_norm launch");
+}
+
+size_t dn_block_norm_bwd_workspace_bytes(const dn_block_norm_bwd_args* a) {
+  return check_block_norm_bwd(a) ? 0 : block_norm_bwd_workspace(*a);
+}
+
+int dn_block_norm_bwd(const dn_block_norm_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_block_norm_bwd(a)) return rc;
+  const size_t need = block_norm_bwd_workspace(*a);
+  if (a->rows == 0 && !need) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(need, a->workspace, a->workspace_bytes, stream, &ws)) return rc;
+  const hipError_t e = launch_block_norm_bwd(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_block_norm_bwd launch");
+}
+
+int dn_embedding(const dn_embedding_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_embedding(a)) return rc;
+  if (a->tokens == 0) return DN_OK;
+  const hipError_t e = launch_embedding(*a, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_embedding launch");
+}
+
+size_t dn_embedding_bwd_workspace_bytes(const dn_embedding_bwd_args* a) {
+  return check_embedding_bwd(a) ? 0 : embedding_bwd_workspace(*a);
+}
+
+int dn_embedding_bwd(const dn_embedding_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_embedding_bwd(a)) return rc;
+  void* ws = nullptr;
+  if (int rc = workspace_for(embedding_bwd_workspace(*a), a->workspace, a->workspace_bytes, stream,
+                             &ws))
+    return rc;
+  const hipError_t e = launch_embedding_bwd(*a, ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_embedding_bwd launch");
+}
+
+size_t dn_attention_workspace_bytes(const dn_attention_args* a) {
+  return check_attention(a) || a->tokens == 0 ? 0 : attention_workspace(*a);
+}
+
+int dn_attention(const dn_attention_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_attention(a)) return rc;
+  if (a->tokens == 0) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(attention_workspace(*a), a->workspace, a->workspace_bytes, stream,
+                             &ws))
+    return rc;
+  const hipError_t e = launch_attention(*a, attention_scale(a->scale, a->head_dim), ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_attention launch");
+}
+
+size_t dn_attention_bwd_workspace_bytes(const dn_attention_bwd_args* a) {
+  return check_attention_bwd(a) || a->tokens == 0 ? 0 : attention_bwd_workspace(*a);
+}
+
+int dn_attention_bwd(const dn_attention_bwd_args* a, hipStream_t stream) {
+  g_last_error.clear();
+  if (int rc = check_attention_bwd(a)) return rc;
+  if (a->tokens == 0 || (!a->d_q && !a->d_k && !a->d_v)) return DN_OK;
+  void* ws = nullptr;
+  if (int rc = workspace_for(attention_bwd_workspace(*a), a->workspace, a->workspace_bytes, stream,
+                             &ws))
+    return rc;
+  const hipError_t e =
+      launch_attention_bwd(*a, attention_scale(a->scale, a->head_dim), ws, stream);
+  return e == hipSuccess ? DN_OK : hip_fail(e, "dn_attention_bwd launch");
+}
+
 int dn_block_step(const dn_block_step_args* a, hipStream_t stream) {
   g_last_error.clear();
   if (!a) return fail(DN_ERR_NULL, "args is NULL");

@@ -1,0 +1,337 @@
+// dn_attention: out = softmax(scale · q kᵀ) v with grouped heads over packed
+// sequences, causal or not, in one pass over the keys.
+//
+// A workgroup takes a tile of rows, a row being one head of one token, the heads
+// of a group side by side: the group's keys are read once for all of them, and one
+// token's heads fill a part of a tile. Its four waves have E rows each and walk the
+// keys in tiles that go through registers into LDS, the next tile's words in flight
+// during the products of this one. Scores are K·Qᵀ, a lane holds scores of one row:
+// the running maximum is its own, and the sums of its two (four) lanes meet at the
+// end. The maximum is followed in steps: the sums are rescaled where it has grown by
+// more than 2^8, which few tiles do after the first, and the weights are below 2^8
+// then.
+//
+// Where there are few tiles of rows the keys are split too; parts meet in the
+// workspace with their maxima and sums, and a second kernel adds them in order.
+//
+// Sums, statistics and scores are fp32; in bf16 the weights are rounded for the
+// matrix unit (their sum is not), the output once.
+#include <algorithm>
+
+#include "attention.hpp"
+#include "layer.hpp"
+
+namespace dn {
+namespace {
+
+using namespace attn;
+
+struct FwdArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  float* part;      // [splits][rows][dim], null: not split
+  float2* part_ml;  // [splits][rows] maximum (in powers of two) and sum
+  Spans spans;
+  Group group;
+  int64_t ldq, ldk, ldv, ldo;
+  int kv_heads, dim, causal, tiles, splits;
+  float c;  // scale · log2(e)
+};
+
+constexpr float kGrowth = 8.f;
+
+template <class T, int HD>
+struct FwdShape {
+  static constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // keys of a tile
+  static constexpr int kBM = 4 * Mma<T>::kE;            // rows of a workgroup
+  static constexpr int kTileWords = kBN * Tile<T, HD>::kWords;
+};
+
+template <class T, int HD>
+__global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdArgs p) {
+  using M = Mma<T>;
+  using S = FwdShape<T, HD>;
+  using Acc = typename M::Acc;
+  constexpr int E = M::kE, BN = S::kBN, KB = BN / E, DB = HD / E, KS = HD / 16;
+  __shared__ uint4 smem[4 * S::kTileWords];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % E, h = lane / E;
+  const int G = p.group.size, heads = G * p.kv_heads;
+  // Heads are the fastest: a head's tiles go to few XCDs, which then share its keys
+  // in their L2. The last tiles, which see the most keys, come first.
+  const int head = int(blockIdx.x) % p.kv_heads;
+  Seq seq;
+  if (!find_tile(p.spans, p.tiles - 1 - int(blockIdx.x) / p.kv_heads, G, S::kBM, &seq)) return;
+  const int rows = seq.len * G, r0 = seq.tile * S::kBM, shift = seq.keys - seq.len;
+  // Keys that any row of the tile sees, and that all do.
+  int some = seq.keys, all = seq.keys;
+  if (p.causal) {
+    some = min(seq.keys, max(0, p.group.token(min(rows, r0 + S::kBM) - 1) + shift + 1));
+    all = min(seq.keys, max(0, p.group.token(r0) + shift + 1));
+  }
+  const int count = (some + BN - 1) / BN, per = (count + p.splits - 1) / p.splits;
+  const int n0 = min(count, int(blockIdx.y) * per), n1 = min(count, n0 + per);
+
+  const int r = r0 + wave * E + c;
+  const bool active = r0 + wave * E < rows, mine = r < rows;  // active: the whole wave
+  const int token = p.group.token(min(r, rows - 1));
+  const int last = p.causal ? min(seq.keys - 1, token + shift) : seq.keys - 1;
+  const int64_t at = int64_t(seq.q0 + token) * heads + head * G + (min(r, rows - 1) - token * G);
+  const Rows<T> ks{static_cast<const T*>(p.k) + int64_t(seq.k0) * p.ldk + int64_t(head) * p.dim,
+                   p.ldk, p.dim, Group{1, 0, 0}};
+  const Rows<T> vs{static_cast<const T*>(p.v) + int64_t(seq.k0) * p.ldv + int64_t(head) * p.dim,
+                   p.ldv, p.dim, Group{1, 0, 0}};
+
+  uint4 q[KS];
+  {
+    const T* row = static_cast<const T*>(p.q) + int64_t(seq.q0 + token) * p.ldq +
+                   int64_t(head * G + (min(r, rows - 1) - token * G)) * p.dim;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = row_word(row, s * 16 + h * M::kCh, p.dim);
+  }
+  Acc o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < M::kAcc; ++i) o[b][i] = 0.f;
+  float top = -INFINITY, sum = 0.f;  // the maximum is in units of scores
+
+  Stage<T, HD, BN, kNT> sk, sv;
+  auto tile_k = [&](int n) { return smem + (n & 1) * 2 * S::kTileWords; };
+  auto tile_v = [&](int n) { return tile_k(n) + S::kTileWords; };
+  // A tile that a row sees in part: whether its values hold anything not finite.
+  auto partly = [&](int n) { return p.causal && (n + 1) * BN > all; };
+  int wild = 0;
+  if (n0 < n1) {
+    const int there = min(BN, seq.keys - n0 * BN);
+    sk.load(ks, n0 * BN, there);
+    sv.load(vs, n0 * BN, there);
+    sk.store(tile_k(n0), there);
+    sv.store(tile_v(n0), there);
+    if (partly(n0)) wild = __syncthreads_or(sv.wild(there));
+    else __syncthreads();
+  }
+  for (int n = n0; n < n1; ++n) {
+    const int there = min(BN, seq.keys - (n + 1) * BN);
+    if (n + 1 < n1) {
+      sk.load(ks, (n + 1) * BN, there);
+      sv.load(vs, (n + 1) * BN, there);
+    }
+    if (wild)  // whole workgroups
+      set_apart<T, HD, BN, kNT, DB>(tile_v(n), o, h, [&](int j) { return n * BN + j <= last; });
+    if (active) {
+      Acc s[KB];
+      const uint4* tk = tile_k(n);
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+#pragma unroll
+        for (int i = 0; i < M::kAcc; ++i) s[b][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) M::mul(Tile<T, HD>::rows(tk, b, k, c, h), q[k], s[b]);
+      }
+      if ((n + 1) * BN > all) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+          for (int i = 0; i < M::kAcc; ++i)
+            s[b][i] = n * BN + b * E + M::row(i, h) <= last ? s[b][i] : -INFINITY;
+      }
+      float m = s[0][0];
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int i = 0; i < M::kAcc; ++i) m = fmaxf(m, s[b][i]);
+#pragma unroll
+      for (int w = E; w < 64; w *= 2) m = fmaxf(m, __shfl_xor(m, w));
+      if (__any(m * p.c > top + kGrowth)) {
+        const float now = fmaxf(top, m * p.c);
+        const float f = now == top ? 1.f : __builtin_amdgcn_exp2f(top - now);
+        top = now;
+        sum *= f;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int i = 0; i < M::kAcc; ++i) o[b][i] *= f;
+      }
+      // No key seen yet: the scores are −inf, and so are these exponents.
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int i = 0; i < M::kAcc; ++i) {
+          s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, -base));
+          sum += s[b][i];
+        }
+      const uint4* tv = tile_v(n);
+      gemm::each<BN / 16>([&](auto step) {
+        constexpr int st = decltype(step)::value;
+        const uint4 w = M::template operand<st>(s);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) M::mul(Tile<T, HD>::cols(tv, b, st, lane), w, o[b]);
+      });
+    }
+    if (n + 1 < n1) {
+      sk.store(tile_k(n + 1), there);
+      sv.store(tile_v(n + 1), there);
+      if (partly(n + 1)) wild = __syncthreads_or(sv.wild(there));
+      else __syncthreads();
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int w = E; w < 64; w *= 2) sum += __shfl_xor(sum, w);
+  if (!mine) return;
+  if (p.part) {
+    const int64_t all_rows = int64_t(p.spans.tokens) * heads, to = blockIdx.y * all_rows + at;
+    if (h == 0) p.part_ml[to] = make_float2(top, sum);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < M::kAcc; ++i) {
+        const int col = b * E + M::row(i, h);
+        if (col < p.dim) p.part[to * p.dim + col] = o[b][i];
+      }
+    return;
+  }
+  // A row that sees no key: zeros, and a log-sum of −inf. NaN stays.
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  T* out = static_cast<T*>(p.out) + int64_t(seq.q0 + token) * p.ldo +
+           int64_t(at - int64_t(seq.q0 + token) * heads) * p.dim;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < M::kAcc; i += 4) {
+      const int col = b * E + M::row(i, h);
+      if (col + 4 <= p.dim) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 w = make_uint2(pk_bf16(o[b][i] * inv, o[b][i + 1] * inv),
+                                     pk_bf16(o[b][i + 2] * inv, o[b][i + 3] * inv));
+          __builtin_memcpy(out + col, &w, 8);
+        } else {
+          const float4 w = make_float4(o[b][i] * inv, o[b][i + 1] * inv, o[b][i + 2] * inv,
+                                       o[b][i + 3] * inv);
+          __builtin_memcpy(out + col, &w, 16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < p.dim) st(out, size_t(col + j), o[b][i + j] * inv);
+      }
+    }
+  if (p.lse && h == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) / kLog2E;
+}
+
+// The parts of a row: a wave a row, 64 columns at a time.
+template <class T>
+__global__ __launch_bounds__(kNT) void attention_join_kernel(FwdArgs p) {
+  const int heads = p.group.size * p.kv_heads, lane = threadIdx.x & 63;
+  const int64_t rows = int64_t(p.spans.tokens) * heads;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 64) top = fmaxf(top, p.part_ml[s * rows + row].x);
+#pragma unroll
+  for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int s = lane; s < p.splits; s += 64) {
+    const float2 ml = p.part_ml[s * rows + row];
+    sum += ml.y * __builtin_amdgcn_exp2f(ml.x - base);
+  }
+#pragma unroll
+  for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const int64_t token = row / heads;
+  T* out = static_cast<T*>(p.out) + token * p.ldo + (row - token * heads) * p.dim;
+  for (int col = lane; col < p.dim; col += 64) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float f = __builtin_amdgcn_exp2f(p.part_ml[s * rows + row].x - base);
+      v += p.part[(s * rows + row) * p.dim + col] * f;
+    }
+    st(out, size_t(col), v * inv);
+  }
+  if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) / kLog2E;
+}
+
+int padded_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+int64_t tile_rows(int dtype) {
+  return 4 * (dtype == DN_BF16 ? Mma<bf16>::kE : Mma<float>::kE);
+}
+
+// Parts of the keys: none where the tiles of rows fill the CUs twice, else as many as
+// do, of at least 256 keys each on average.
+int splits_of(const dn_attention_args& a) {
+  const int64_t group = a.nheads / a.kv_heads;
+  const int64_t tiles =
+      std::max<int64_t>(a.sequences, a.tokens * group / tile_rows(a.dtype)) * a.kv_heads;
+  const int64_t want = 2 * device_cu_count() / std::max<int64_t>(1, tiles);
+  const int64_t keys = a.key_starts ? a.key_rows : a.tokens;
+  const int64_t most = keys / std::max<int64_t>(1, a.sequences) / 256;
+  return int(std::max<int64_t>(1, std::min<int64_t>({want, most, 256})));
+}
+
+template <class T, int HD>
+hipError_t fwd_go(const FwdArgs& p, hipStream_t stream) {
+  const auto fn = attention_kernel<T, HD>;
+  {
+    ProfScope ps("dn_attention", stream);
+    hipLaunchKernelGGL(fn, dim3(unsigned(p.tiles) * unsigned(p.kv_heads), unsigned(p.splits)),
+                       dim3(kNT), 0, stream, p);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !p.part) return e;
+  ProfScope ps("dn_attention_join", stream);
+  const int64_t rows = int64_t(p.spans.tokens) * p.group.size * p.kv_heads;
+  hipLaunchKernelGGL((attention_join_kernel<T>), dim3(unsigned((rows + 3) / 4)), dim3(kNT), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+template <class T>
+hipError_t fwd_typed(const FwdArgs& p, hipStream_t stream) {
+  const int hd = padded_dim(p.dim);
+  return hd == 64    ? fwd_go<T, 64>(p, stream)
+         : hd == 128 ? fwd_go<T, 128>(p, stream)
+                     : fwd_go<T, 256>(p, stream);
+}
+
+}  // namespace
+
+size_t attention_workspace(const dn_attention_args& a) {
+  const size_t splits = size_t(splits_of(a)), rows = size_t(a.tokens) * size_t(a.nheads);
+  if (splits == 1) return 0;
+  return align_up(splits * rows * size_t(a.head_dim) * 4, 256) + splits * rows * sizeof(float2);
+}
+
+hipError_t launch_attention(const dn_attention_args& a, float scale, void* ws, hipStream_t stream) {
+  FwdArgs p{};
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.group = group_of(a.nheads / a.kv_heads);
+  p.spans = {a.offsets, a.key_starts, a.key_lengths, int(a.sequences), int(a.tokens),
+             int(a.key_starts ? a.key_rows : a.tokens),
+             int(a.sequences ? a.tokens / a.sequences : 0)};
+  p.ldq = a.q_stride;
+  p.ldk = a.k_stride;
+  p.ldv = a.v_stride;
+  p.ldo = a.out_stride;
+  p.kv_heads = int(a.kv_heads);
+  p.dim = int(a.head_dim);
+  p.causal = a.causal;
+  p.tiles = int(tile_count(a.tokens, p.group.size, tile_rows(a.dtype), a.sequences));
+  p.splits = splits_of(a);
+  p.c = scale * kLog2E;
+  if (p.splits > 1) {
+    const size_t rows = size_t(a.tokens) * size_t(a.nheads);
+    p.part = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(
+        static_cast<char*>(ws) + align_up(size_t(p.splits) * rows * size_t(a.head_dim) * 4, 256));
+  }
+  return a.dtype == DN_BF16 ? fwd_typed<bf16>(p, stream) : fwd_typed<float>(p, stream);
+}
+
+}  // namespace dn

@@ -35,4 +35,18 @@ hipError_t launch_gated_ffn(const dn_gated_ffn_args& a, void* ws, hipStream_t st
 size_t gated_ffn_bwd_workspace(const dn_gated_ffn_bwd_args& a);
 hipError_t launch_gated_ffn_bwd(const dn_gated_ffn_bwd_args& a, void* ws, hipStream_t stream);
 
+// Between token ids and logits (block_norm.hip, embedding.hip, attention.hip,
+// attention_bwd.hip).
+hipError_t launch_block_norm(const dn_block_norm_args& a, hipStream_t stream);
+size_t block_norm_bwd_workspace(const dn_block_norm_bwd_args& a);
+hipError_t launch_block_norm_bwd(const dn_block_norm_bwd_args& a, void* ws, hipStream_t stream);
+hipError_t launch_embedding(const dn_embedding_args& a, hipStream_t stream);
+size_t embedding_bwd_workspace(const dn_embedding_bwd_args& a);
+hipError_t launch_embedding_bwd(const dn_embedding_bwd_args& a, void* ws, hipStream_t stream);
+size_t attention_workspace(const dn_attention_args& a);
+hipError_t launch_attention(const dn_attention_args& a, float scale, void* ws, hipStream_t stream);
+size_t attention_bwd_workspace(const dn_attention_bwd_args& a);
+hipError_t launch_attention_bwd(const dn_attention_bwd_args& a, float scale, void* ws,
+                                hipStream_t stream);
+
 }  // namespace dn

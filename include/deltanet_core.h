@@ -547,6 +547,136 @@ typedef struct {
 int dn_gated_ffn_bwd(const dn_gated_ffn_bwd_args *args, hipStream_t stream);
 size_t dn_gated_ffn_bwd_workspace_bytes(const dn_gated_ffn_bwd_args *args);
 
+/* What joins a block and the residual stream: with u = x / sqrt(mean(x^2) + eps) *
+ * post_weight (u = x without post_weight), sum = residual_scale * residual + gate * u
+ * and out = sum / sqrt(mean(sum^2) + eps) * pre_weight, from the unrounded sum. */
+typedef enum {
+  DN_GATE_NONE = 0,
+  DN_GATE_CHANNEL = 1, /* [dim], weight_dtype */
+  DN_GATE_TOKEN = 2,   /* a value a row, gate_stride apart, dtype */
+  DN_GATE_FULL = 3     /* [rows, dim], dtype */
+} dn_gate_kind;
+
+typedef struct {
+  int64_t rows, dim;
+  int64_t x_stride, residual_stride, gate_stride, sum_stride, out_stride;
+  double eps, residual_scale;
+  int32_t dtype;           /* x, residual, sum, out: DN_F32 or DN_BF16 */
+  int32_t weight_dtype;    /* pre_weight, post_weight */
+  int32_t gate_kind;
+  const void *x, *residual;
+  const void *pre_weight;  /* [dim] */
+  const void *post_weight; /* [dim]; NULL: no norm after the block */
+  const void *gate;        /* NULL for DN_GATE_NONE */
+  void *sum;               /* may alias x or residual */
+  void *out;
+} dn_block_norm_args;
+
+int dn_block_norm(const dn_block_norm_args *args, hipStream_t stream);
+
+/* Its gradients at `sum` (as the forward wrote it); each may be left out (NULL).
+ * d_gate has the gate's kind, layout and dtype. The column sums are added up in a
+ * fixed order. */
+typedef struct {
+  int64_t rows, dim;
+  int64_t x_stride, sum_stride, gate_stride, d_out_stride, d_sum_stride;
+  int64_t d_x_stride, d_residual_stride, d_gate_stride;
+  double eps, residual_scale;
+  int32_t dtype, weight_dtype, gate_kind;
+  const void *x, *sum, *pre_weight, *post_weight, *gate;
+  const void *d_out, *d_sum; /* NULL: zeros */
+  void *d_x, *d_residual, *d_pre_weight, *d_post_weight, *d_gate;
+  void *workspace;           /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_block_norm_bwd_args;
+
+int dn_block_norm_bwd(const dn_block_norm_bwd_args *args, hipStream_t stream);
+size_t dn_block_norm_bwd_workspace_bytes(const dn_block_norm_bwd_args *args);
+
+/* out[i] = scale * table[ids[i]]; an id outside [0, vocab) stands for a row of
+ * zeros. Up to 2^28 tokens, a vocab up to 2^24. */
+typedef struct {
+  int64_t tokens, vocab, dim;
+  int64_t table_stride, out_stride;
+  double scale;
+  int32_t dtype;    /* table, out: DN_F32 or DN_BF16 */
+  int32_t wide_ids; /* ids are int64 (else int32) */
+  const void *ids;  /* [tokens] */
+  const void *table;
+  void *out;
+} dn_embedding_args;
+
+int dn_embedding(const dn_embedding_args *args, hipStream_t stream);
+
+/* The table's gradient, written whole: d_table[v] = scale * the sum of d_out[i] over
+ * the tokens with ids[i] = v, added up in a fixed order. Ids outside [0, vocab) take
+ * no part. */
+typedef struct {
+  int64_t tokens, vocab, dim;
+  int64_t d_out_stride, d_table_stride;
+  double scale;
+  int32_t dtype, wide_ids;
+  const void *ids, *d_out;
+  void *d_table;
+  void *workspace; /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_embedding_bwd_args;
+
+int dn_embedding_bwd(const dn_embedding_bwd_args *args, hipStream_t stream);
+size_t dn_embedding_bwd_workspace_bytes(const dn_embedding_bwd_args *args);
+
+/* Softmax attention over packed sequences: out = softmax(scale q k^T) v for each of
+ * nheads heads; kv_heads divides nheads, head h reads key head h / (nheads/kv_heads).
+ *   q, out  [tokens, nheads, head_dim]     k, v  [key_rows, kv_heads, head_dim]
+ * a token's heads side by side, *_stride elements between tokens. Sequence s has the
+ * query rows [offsets[s], offsets[s+1]); offsets (int32, on the device) start at 0 and
+ * do not fall; NULL: `sequences` of tokens / sequences rows each. Its keys are the same
+ * rows of k and v, or key_lengths[s] rows from key_starts[s] on (a cache; spans may
+ * overlap). Causal: the i-th of n queries over m keys sees keys 0 ... i + m - n. A row
+ * that sees no key, and every row behind the last sequence, gets zeros, and -inf as its
+ * log-sum. Keys that a row does not see have no influence on it, whatever they hold;
+ * offsets and spans that leave the tensors are cut off at their ends. Scores, sums and
+ * statistics are fp32. head_dim up to 256; (tokens + sequences) * nheads below 2^31. */
+typedef struct {
+  int64_t tokens, key_rows, sequences, nheads, kv_heads, head_dim;
+  int64_t q_stride, k_stride, v_stride, out_stride;
+  double scale;   /* above 0; NaN: 1/sqrt(head_dim) */
+  int32_t dtype;  /* q, k, v, out: DN_F32 or DN_BF16 */
+  int32_t causal;
+  const void *q, *k, *v;
+  const int32_t *offsets;
+  const int32_t *key_starts, *key_lengths; /* [sequences], or both NULL */
+  void *out;
+  float *lse;     /* [tokens, nheads]: the natural log of the sum of exp(scale q k); or NULL */
+  void *workspace; /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_attention_args;
+
+int dn_attention(const dn_attention_args *args, hipStream_t stream);
+size_t dn_attention_workspace_bytes(const dn_attention_args *args);
+
+/* Its gradients where every sequence's keys are its own rows, from the forward's out
+ * and lse; each may be left out (NULL). Rows behind the last sequence get zeros. Every
+ * gradient is summed in a fixed order. */
+typedef struct {
+  int64_t tokens, sequences, nheads, kv_heads, head_dim;
+  int64_t q_stride, k_stride, v_stride, out_stride, d_out_stride;
+  int64_t d_q_stride, d_k_stride, d_v_stride;
+  double scale;
+  int32_t dtype, causal;
+  const void *q, *k, *v;
+  const int32_t *offsets;
+  const void *out;
+  const float *lse;
+  const void *d_out;
+  void *d_q, *d_k, *d_v;
+  void *workspace; /* NULL: library-managed */
+  size_t workspace_bytes;
+} dn_attention_bwd_args;
+
+int dn_attention_bwd(const dn_attention_bwd_args *args, hipStream_t stream);
+size_t dn_attention_bwd_workspace_bytes(const dn_attention_bwd_args *args);
+
 /* How unit_lower_inverse inverts I − N (TriSolve, src/delta/tri.rs:53-64). */
 typedef enum {
   DN_TRI_BLOCKED = 0, /* the exact inverse without powers of N (the default) */
