@@ -1241,8 +1241,9 @@ int check_heads(int64_t tokens, int64_t sequences, int64_t nheads, int64_t kv_he
   if (nheads > 65536 || tokens > INT32_MAX / 2 || sequences > INT32_MAX / 2 ||
       (tokens + sequences) * nheads > INT32_MAX / 2)
     return fail(DN_ERR_SHAPE, "tensor too large");
-  // A launch has fewer than 2^32 threads: tiles of 64 rows at the least.
-  if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 24))
+  // A launch has fewer than 2^32 threads: tiles of 64 rows at the least, two workgroups
+  // of 256 threads to a tile of keys.
+  if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 23))
     return fail(DN_ERR_SHAPE, "tensor too large");
   if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
   if (!std::isnan(scale) && !(scale > 0.0 && float(scale) > 0.f && std::isfinite(float(scale))))

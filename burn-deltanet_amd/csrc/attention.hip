@@ -36,6 +36,7 @@ struct FwdArgs {
   Group group;
   int64_t ldq, ldk, ldv, ldo;
   int kv_heads, dim, causal, tiles, splits;
+  bool words;  // keys and values lie in whole words
   float c;  // scale · log2(e)
 };
 
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
   using S = FwdShape<T, HD>;
   using Acc = typename M::Acc;
   constexpr int E = M::kE, BN = S::kBN, KB = BN / E, DB = HD / E, KS = HD / 16;
-  __shared__ uint4 smem[4 * S::kTileWords];
+  __shared__ uint4 smem[4 * S::kTileWords];  // keys, values; of two tiles
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % E, h = lane / E;
   const int G = p.group.size, heads = G * p.kv_heads;
   // Heads are the fastest: a head's tiles go to few XCDs, which then share its keys
@@ -77,11 +78,25 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
   const int token = p.group.token(min(r, rows - 1));
   const int last = p.causal ? min(seq.keys - 1, token + shift) : seq.keys - 1;
   const int64_t at = int64_t(seq.q0 + token) * heads + head * G + (min(r, rows - 1) - token * G);
-  const Rows<T> ks{static_cast<const T*>(p.k) + int64_t(seq.k0) * p.ldk + int64_t(head) * p.dim,
-                   p.ldk, p.dim, Group{1, 0, 0}};
-  const Rows<T> vs{static_cast<const T*>(p.v) + int64_t(seq.k0) * p.ldv + int64_t(head) * p.dim,
-                   p.ldv, p.dim, Group{1, 0, 0}};
-
+  const Feed<T, HD, BN> keys(
+      Rows<T>{static_cast<const T*>(p.k) + int64_t(seq.k0) * p.ldk + int64_t(head) * p.dim, p.ldk,
+              p.dim, Group{1, 0, 0}},
+      p.words);
+  const Feed<T, HD, BN> values(
+      Rows<T>{static_cast<const T*>(p.v) + int64_t(seq.k0) * p.ldv + int64_t(head) * p.dim, p.ldv,
+              p.dim, Group{1, 0, 0}},
+      p.words);
+  const Reader<T, HD> read(lane);
+  auto load = [&](int n, int buf) {
+    const int there = min(BN, seq.keys - n * BN);
+    keys.load(smem + buf * 2 * S::kTileWords, n * BN, there);
+    values.load(smem + (buf * 2 + 1) * S::kTileWords, n * BN, there);
+  };
+  if (n0 < n1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keys.clear_rest(smem + i * S::kTileWords);
+    load(n0, 0);
+  }
   uint4 q[KS];
   {
     const T* row = static_cast<const T*>(p.q) + int64_t(seq.q0 + token) * p.ldq +
@@ -94,42 +109,32 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int i = 0; i < M::kAcc; ++i) o[b][i] = 0.f;
-  float top = -INFINITY, sum = 0.f;  // the maximum is in units of scores
+  float top = -INFINITY, sum = 0.f;  // the maximum in powers of two
+  feed_barrier();
 
-  Stage<T, HD, BN, kNT> sk, sv;
-  auto tile_k = [&](int n) { return smem + (n & 1) * 2 * S::kTileWords; };
-  auto tile_v = [&](int n) { return tile_k(n) + S::kTileWords; };
-  // A tile that a row sees in part: whether its values hold anything not finite.
-  auto partly = [&](int n) { return p.causal && (n + 1) * BN > all; };
-  int wild = 0;
-  if (n0 < n1) {
-    const int there = min(BN, seq.keys - n0 * BN);
-    sk.load(ks, n0 * BN, there);
-    sv.load(vs, n0 * BN, there);
-    sk.store(tile_k(n0), there);
-    sv.store(tile_v(n0), there);
-    if (partly(n0)) wild = __syncthreads_or(sv.wild(there));
-    else __syncthreads();
-  }
-  for (int n = n0; n < n1; ++n) {
-    const int there = min(BN, seq.keys - (n + 1) * BN);
-    if (n + 1 < n1) {
-      sk.load(ks, (n + 1) * BN, there);
-      sv.load(vs, (n + 1) * BN, there);
+  // Tile n in buffer `parity`; one that a row sees in part (`partly`), or whole.
+  auto step = [&](auto parity, auto partly, int n) {
+    constexpr int buf = decltype(parity)::value;
+    constexpr bool kPartly = decltype(partly)::value;
+    uint4* const value_tile = smem + (buf * 2 + 1) * S::kTileWords;
+    const char* const tk = reinterpret_cast<const char*>(smem + buf * 2 * S::kTileWords);
+    const char* const tv = reinterpret_cast<const char*>(value_tile);
+    if constexpr (kPartly) {
+      if (__syncthreads_or(Feed<T, HD, BN>::wild(value_tile)))
+        set_apart<T, HD, BN, kNT, DB>(value_tile, o, h, [&](int j) { return n * BN + j <= last; });
     }
-    if (wild)  // whole workgroups
-      set_apart<T, HD, BN, kNT, DB>(tile_v(n), o, h, [&](int j) { return n * BN + j <= last; });
+    if (n + 1 < n1) load(n + 1, buf ^ 1);
     if (active) {
       Acc s[KB];
-      const uint4* tk = tile_k(n);
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < M::kAcc; ++i) s[b][i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) M::mul(Tile<T, HD>::rows(tk, b, k, c, h), q[k], s[b]);
-      }
-      if ((n + 1) * BN > all) {
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int b = 0; b < KB; ++b) M::mul(read.rows(tk, b, k), q[k], s[b]);
+      if constexpr (kPartly) {
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -141,10 +146,9 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < M::kAcc; ++i) m = fmaxf(m, s[b][i]);
-#pragma unroll
-      for (int w = E; w < 64; w *= 2) m = fmaxf(m, __shfl_xor(m, w));
-      if (__any(m * p.c > top + kGrowth)) {
-        const float now = fmaxf(top, m * p.c);
+      m = over_column<E>(m, [](float x, float y) { return fmaxf(x, y); }) * p.c;
+      if (__any(m > top + kGrowth)) {
+        const float now = fmaxf(top, m);
         const float f = now == top ? 1.f : __builtin_amdgcn_exp2f(top - now);
         top = now;
         sum *= f;
@@ -162,24 +166,19 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
           s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, -base));
           sum += s[b][i];
         }
-      const uint4* tv = tile_v(n);
-      gemm::each<BN / 16>([&](auto step) {
-        constexpr int st = decltype(step)::value;
-        const uint4 w = M::template operand<st>(s);
 #pragma unroll
-        for (int b = 0; b < DB; ++b) M::mul(Tile<T, HD>::cols(tv, b, st, lane), w, o[b]);
-      });
+      for (int st = 0; st < BN / 16; ++st) {
+        const uint4 w = M::operand(s[st / M::kHalves], st % M::kHalves);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) M::mul(read.cols(tv, b, st), w, o[b]);
+      }
     }
-    if (n + 1 < n1) {
-      sk.store(tile_k(n + 1), there);
-      sv.store(tile_v(n + 1), there);
-      if (partly(n + 1)) wild = __syncthreads_or(sv.wild(there));
-      else __syncthreads();
-    }
-  }
+    feed_barrier();
+  };
+  walk(all / BN - n0, n1 - n0,
+       [&](auto parity, auto partly, int n) { step(parity, partly, n0 + n); });
   if (!active) return;
-#pragma unroll
-  for (int w = E; w < 64; w *= 2) sum += __shfl_xor(sum, w);
+  sum = over_column<E>(sum, [](float x, float y) { return x + y; });
   if (!mine) return;
   if (p.part) {
     const int64_t all_rows = int64_t(p.spans.tokens) * heads, to = blockIdx.y * all_rows + at;
@@ -325,6 +324,7 @@ hipError_t launch_attention(const dn_attention_args& a, float scale, void* ws, h
   p.tiles = int(tile_count(a.tokens, p.group.size, tile_rows(a.dtype), a.sequences));
   p.splits = splits_of(a);
   p.c = scale * kLog2E;
+  p.words = in_words(a.dtype, p.dim, {{a.k, p.ldk}, {a.v, p.ldv}});
   if (p.splits > 1) {
     const size_t rows = size_t(a.tokens) * size_t(a.nheads);
     p.part = static_cast<float*>(ws);

@@ -14,6 +14,8 @@
 // values of the contraction, one word a lane.
 #pragma once
 
+#include <initializer_list>
+
 #include "dn_common.hpp"
 #include "gemm.hpp"
 #include "mfma_util.hpp"
@@ -22,6 +24,9 @@ namespace dn {
 namespace attn {
 
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kNT = 256;  // threads of a workgroup: four waves
 
 template <class T>
 struct Mma;
@@ -36,11 +41,10 @@ struct Mma<bf16> {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  // Rows 16·s … of a column of blocks as an operand.
-  template <int S, int N>
-  static __device__ inline uint4 operand(const Acc (&x)[N]) {
-    const Acc& a = x[S / 2];
-    constexpr int o = 8 * (S & 1);
+  // Rows 16·half … of a block as an operand.
+  static constexpr int kHalves = 2;
+  static __device__ inline uint4 operand(const Acc& a, int half) {
+    const int o = 8 * half;
     return make_uint4(pk_bf16(a[o], a[o + 1]), pk_bf16(a[o + 2], a[o + 3]),
                       pk_bf16(a[o + 4], a[o + 5]), pk_bf16(a[o + 6], a[o + 7]));
   }
@@ -70,10 +74,8 @@ struct Mma<float> {
     c = mfma_f32(__uint_as_float(a.z), __uint_as_float(b.z), c);
     c = mfma_f32(__uint_as_float(a.w), __uint_as_float(b.w), c);
   }
-  template <int S, int N>
-  static __device__ inline uint4 operand(const Acc (&x)[N]) {
-    return __builtin_bit_cast(uint4, x[S]);
-  }
+  static constexpr int kHalves = 1;
+  static __device__ inline uint4 operand(const Acc& a, int) { return __builtin_bit_cast(uint4, a); }
   template <int HD>
   static __device__ inline int spread(int row) {
     return row & 15;
@@ -91,36 +93,6 @@ struct Tile {
   static constexpr int kWords = HD / M::kCh;  // of a row
   static __device__ inline int at(int row, int word) {
     return row * kWords + (word ^ M::template spread<HD>(row));
-  }
-  // Rows E·blk …, values 16·step … of them.
-  static __device__ inline uint4 rows(const uint4* t, int blk, int step, int c, int h) {
-    return t[at(blk * M::kE + c, step * (16 / M::kCh) + h)];
-  }
-  // Columns E·blk … as rows, contraction over rows 16·step … in the order of an
-  // accumulator's registers.
-  static __device__ inline uint4 cols(const uint4* t, int blk, int step, int lane) {
-    if constexpr (sizeof(T) == 2) {
-      // Lane i of a 16-lane group names four columns of row i / 4, and receives
-      // column i of those four rows.
-      const int i = lane & 15, g = lane >> 4;
-      const int row = 16 * step + 4 * (g >> 1) + (i >> 2);
-      const int col = 32 * blk + 16 * (g & 1) + 4 * (i & 3);
-      typedef short v4s __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) v4s* P;
-      const char* p = reinterpret_cast<const char*>(t) + (col & 7) * 2;
-      const uint2 lo = __builtin_bit_cast(
-          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 16 * at(row, col >> 3))));
-      const uint2 hi = __builtin_bit_cast(
-          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 16 * at(row + 8, col >> 3))));
-      return make_uint4(lo.x, lo.y, hi.x, hi.y);
-    } else {
-      const int c = lane & 15, h = lane >> 4, col = 16 * blk + c;
-      auto one = [&](int r) {
-        return reinterpret_cast<const uint32_t*>(t)[4 * at(16 * step + 4 * h + r, col >> 2) +
-                                                    (col & 3)];
-      };
-      return make_uint4(one(0), one(1), one(2), one(3));
-    }
   }
   static __device__ inline float value(const uint4* t, int row, int col) {
     return ld(reinterpret_cast<const T*>(t + at(row, col / M::kCh)), size_t(col % M::kCh));
@@ -177,53 +149,207 @@ __device__ inline uint4 row_word(const T* row, int col, int dim) {
   return w;
 }
 
-// ROWS rows on their way from memory to LDS through registers.
-template <class T, int HD, int ROWS, int NT>
-struct Stage {
-  static constexpr int kWords = Tile<T, HD>::kWords, kN = ROWS * kWords / NT;
-  static_assert(ROWS * kWords % NT == 0, "whole words a thread");
-  uint4 w[kN];
-  // Rows from `first` on, `there` (at least 1) of them; the others become zeros.
-  __device__ inline void load(const Rows<T>& src, int first, int there) {
-    if (src.dim == HD) {
+// Where a lane's operand words lie in a tile, in bytes: for a block's first words, the
+// others being a constant further.
+template <class T, int HD>
+struct Reader {
+  using M = Mma<T>;
+  using TL = Tile<T, HD>;
+  static constexpr int kSpan = TL::kWords < 16 ? TL::kWords : 16;  // words that `spread` mixes
+  static constexpr int kStepWords = 16 / M::kCh, kSteps = kSpan / kStepWords;
+  static constexpr int kBlkWords = M::kE / M::kCh, kBlks = kSpan / kBlkWords;
+  static constexpr int kParts = sizeof(T) == 2 ? 2 : 4;
+  static constexpr int kRow = TL::kWords * 16;
+  uint32_t row[kSteps], col[kBlks][kParts];
+  __device__ inline explicit Reader(int lane) {
+    const int c = lane % M::kE, h = lane / M::kE;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = i * NT + int(threadIdx.x), r = e / kWords;
-        __builtin_memcpy(&w[i], src.at(first + min(r, there - 1)) + (e % kWords) * Mma<T>::kCh, 16);
+    for (int s = 0; s < kSteps; ++s) row[s] = TL::at(c, s * kStepWords + h) * 16;
+#pragma unroll
+    for (int b = 0; b < kBlks; ++b)
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          // Lane i of a 16-lane group names four columns of row i / 4, and receives
+          // column i of those four rows.
+          const int i = lane & 15, g = lane >> 4;
+          const int r = 4 * (g >> 1) + 8 * j + (i >> 2), x = 32 * b + 16 * (g & 1) + 4 * (i & 3);
+          col[b][j] = TL::at(r, x >> 3) * 16 + (x & 7) * 2;
+        } else {
+          const int x = 16 * b + c;
+          col[b][j] = TL::at(4 * h + j, x >> 2) * 16 + (x & 3) * 4;
+        }
       }
+  }
+  // Rows E·blk …, values 16·step … of them.
+  __device__ inline uint4 rows(const char* t, int blk, int step) const {
+    return *reinterpret_cast<const uint4*>(t + row[step % kSteps] + (step / kSteps) * kSpan * 16 +
+                                           blk * M::kE * kRow);
+  }
+  // Columns E·blk … as rows, contraction over rows 16·step … in the order of an
+  // accumulator's registers.
+  __device__ inline uint4 cols(const char* t, int blk, int step) const {
+    const int far = (blk / kBlks) * kSpan * 16 + step * 16 * kRow;
+    if constexpr (sizeof(T) == 2) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) v4s* P;
+      const uint2 lo = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(t + col[blk % kBlks][0] + far)));
+      const uint2 hi = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(t + col[blk % kBlks][1] + far)));
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
     } else {
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = i * NT + int(threadIdx.x), r = e / kWords;
-        w[i] = row_word(src.at(first + min(r, there - 1)), (e % kWords) * Mma<T>::kCh, src.dim);
-      }
+      auto one = [&](int j) {
+        return *reinterpret_cast<const uint32_t*>(t + col[blk % kBlks][j] + far);
+      };
+      return make_uint4(one(0), one(1), one(2), one(3));
     }
   }
-  __device__ inline void store(uint4* tile, int there) const {
-    if (there >= ROWS) {
+};
+
+__device__ inline uint32_t wave_index() {
+  return uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+}
+// A pointer that is the same in all lanes, in scalar registers.
+__device__ inline const char* scalar(const char* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const char*>(
+      uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(u >> 32)))) << 32 |
+      uint32_t(__builtin_amdgcn_readfirstlane(int(u))));
+}
+
+// Tiles of ROWS rows on their way from memory to LDS. Copies need no registers: they
+// are issued a tile ahead and waited for behind the products. They take whole words at
+// 16-byte steps (`words`); rows that lie otherwise go through registers at once. Where
+// a step of 16 rows is the same distance everywhere (`even`), a whole tile's addresses
+// are a scalar base and an offset of the lane's own that stays.
+template <class T, int HD, int ROWS>
+struct Feed {
+  using M = Mma<T>;
+  using TL = Tile<T, HD>;
+  static constexpr int kN = ROWS * TL::kWords / kNT;  // words of a thread
+  static constexpr int kStep = kNT / TL::kWords;      // rows from one to the next
+  static constexpr int kLong = kStep < 16 ? 16 : kStep, kD = kLong / kStep;
+  static_assert(ROWS * TL::kWords % kNT == 0 && ROWS % kLong == 0, "whole words a thread");
+  Rows<T> src;
+  bool words, even;
+  int64_t far;  // bytes of kLong rows
+  uint32_t off[kD];
+  bool on[kD];
+  __device__ inline Feed(const Rows<T>& rows, bool can_copy) : src(rows), words(can_copy) {
+    const int g = src.group.size;
+    even = 16 % g == 0;
+    far = src.ld * int64_t(sizeof(T)) * (kLong / (even ? g : 1));
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = i * NT + int(threadIdx.x);
-        tile[Tile<T, HD>::at(e / kWords, e % kWords)] = w[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int e = i * NT + int(threadIdx.x);
-        tile[Tile<T, HD>::at(e / kWords, e % kWords)] =
-            e / kWords < there ? w[i] : make_uint4(0, 0, 0, 0);
-      }
+    for (int d = 0; d < kD; ++d) {
+      const int e = d * kNT + int(threadIdx.x), r = e / TL::kWords;
+      const int word = (e % TL::kWords) ^ M::template spread<HD>(r);
+      const int t = even ? src.group.token(r) : 0;
+      off[d] = uint32_t(t) * uint32_t(src.ld * int64_t(sizeof(T))) +
+               uint32_t((r - t * g) * src.dim * int(sizeof(T)) + word * 16);
+      on[d] = word * M::kCh < src.dim;
     }
   }
-  // Whether the rows that are there hold an infinity or a NaN.
-  __device__ inline int wild(int there) const {
+  // Words past the rows' ends, which copies do not write.
+  __device__ inline void clear_rest(uint4* tile) const {
+    if (src.dim == HD) return;
+    for (int e = threadIdx.x; e < ROWS * TL::kWords; e += kNT)
+      if (((e % TL::kWords) ^ M::template spread<HD>(e / TL::kWords)) * M::kCh >= src.dim)
+        tile[e] = make_uint4(0, 0, 0, 0);
+  }
+  // Rows from `first` (a multiple of ROWS) on, `there` (at least 1) of them; the others
+  // become zeros.
+  __device__ inline void load(uint4* tile, int first, int there) const {
+    if (words && even && there >= ROWS) {
+      const char* base = scalar(reinterpret_cast<const char*>(src.base) +
+                                int64_t(first / kLong) * far);
+      const uint32_t to = gemm::lds_address(tile) + wave_index() * 1024;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        if (src.dim == HD)
+          gemm::copy_to_lds(base + (i / kD) * far, off[i % kD], to + i * kNT * 16);
+        else if (on[i % kD])
+          gemm::copy_to_lds(base + (i / kD) * far, off[i % kD], to + i * kNT * 16);
+      }
+    } else {
+      load_any(tile, first, there);
+    }
+  }
+  __device__ inline void load_any(uint4* tile, int first, int there) const {
+    const uint32_t to = gemm::lds_address(tile) + wave_index() * 1024;
+#pragma unroll 1
+    for (int i = 0; i < kN; ++i) {
+      const int e = i * kNT + int(threadIdx.x), r = e / TL::kWords;
+      const int col = ((e % TL::kWords) ^ M::template spread<HD>(r)) * M::kCh;
+      const T* row = src.at(first + min(r, there - 1));
+      if (r >= there || col >= src.dim) tile[e] = make_uint4(0, 0, 0, 0);
+      else if (words) gemm::copy_to_lds(reinterpret_cast<const char*>(row + col), to + i * kNT * 16);
+      else tile[e] = row_word(row, col, src.dim);
+    }
+  }
+  // Whether a tile in LDS holds an infinity or a NaN.
+  static __device__ inline int wild(const uint4* tile) {
     int bad = 0;
-#pragma unroll
-    for (int i = 0; i < kN; ++i)
-      bad |= (i * NT + int(threadIdx.x)) / kWords < there && !Mma<T>::finite(w[i]);
+    for (int i = 0; i < kN; ++i) bad |= !M::finite(tile[i * kNT + int(threadIdx.x)]);
     return bad;
   }
 };
+// This wave's copies have landed and its LDS accesses are done; then all waves'.
+__device__ inline void feed_barrier() {
+  gemm::wait_copies<0>();
+  lds_barrier();
+}
+
+// step(buffer, partly, n) for the tiles 0 … count − 1 of a walk, which take the two
+// buffers in turn: the first `whole` are seen whole and the others in part.
+template <class Step>
+__device__ inline void walk(int whole, int count, Step step) {
+  using A = std::integral_constant<int, 0>;
+  using B = std::integral_constant<int, 1>;
+  for (int n = 0; n < count; n += 2) {
+    if (n < whole) step(A{}, std::false_type{}, n);
+    else step(A{}, std::true_type{}, n);
+    if (n + 1 >= count) break;
+    if (n + 1 < whole) step(B{}, std::false_type{}, n + 1);
+    else step(B{}, std::true_type{}, n + 1);
+  }
+}
+
+// N products in order, with(i, word), the words read from LDS kAhead products ahead, and
+// what `with` does beside its product kept there: a SIMD's vector unit works while its
+// matrix unit does, but each wave hands out its instructions in order. Left to itself
+// the compiler reads every word where it is used and gathers the rest behind.
+template <int N, int kAhead, class Read, class With>
+__device__ inline void in_turn(Read read, With with) {
+  constexpr int kRing = kAhead + 1;
+  uint4 ring[kRing];
+  gemm::each<(kAhead < N ? kAhead : N)>([&](auto i) { ring[decltype(i)::value] = read(i); });
+  gemm::each<N>([&](auto i) {
+    constexpr int at = decltype(i)::value;
+    if constexpr (at + kAhead < N)
+      ring[(at + kAhead) % kRing] = read(std::integral_constant<int, at + kAhead>{});
+    with(i, ring[at % kRing]);
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+// f(e) for the part of [0, TOTAL) that falls to piece I of N.
+template <int TOTAL, int N, int I, class F>
+__device__ inline void share(F f) {
+  constexpr int lo = TOTAL * I / N, hi = TOTAL * (I + 1) / N;
+#pragma unroll
+  for (int e = lo; e < hi; ++e) f(e);
+}
+
+// A value of the E lanes (h) of each column, over them.
+template <int E, class F>
+__device__ inline float over_column(float v, F f) {
+  if constexpr (E == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  }
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
 
 // A tile whose rows do not all count for every column of a product, and that holds
 // infinities or NaN: the matrix unit would carry them into columns that do not see
@@ -304,12 +430,23 @@ __device__ inline bool find_tile(const Spans& sp, int t, int per, int edge, Seq*
   }
   return out->tile >= 0 && int64_t(out->tile) * edge < int64_t(out->len) * per;
 }
+// Whether tensors' rows can be copied to LDS: heads of whole words, at 16-byte steps,
+// with 32-bit offsets between rows of a tile.
+struct Lying {
+  const void* p;
+  int64_t ld;
+};
+inline bool in_words(int dtype, int dim, std::initializer_list<Lying> tensors) {
+  const int64_t size = dtype == DN_BF16 ? 2 : 4;
+  if (dim * size % 16) return false;
+  for (const Lying& t : tensors)
+    if (reinterpret_cast<uintptr_t>(t.p) % 16 || t.ld * size % 16 || t.ld >= (1 << 23)) return false;
+  return true;
+}
 inline int64_t tile_count(int64_t tokens, int64_t per, int64_t edge, int64_t sequences) {
   return tokens * per / edge + sequences + 1;
 }
 
-constexpr float kLog2E = 1.4426950408889634f;
-constexpr int kNT = 256;  // threads of a workgroup: four waves
 
 }  // namespace attn
 }  // namespace dn

@@ -3,8 +3,7 @@
 // and dS = P ⊙ (dP − δ):
 //   d_q = scale·dS k,  d_k = scale·dSᵀ q,  d_v = Pᵀ d_out.
 //
-// Three launches: δ (with lse in powers of two beside it, the rows of a group side by
-// side); d_q, a workgroup a tile of rows that walks the keys; d_k and d_v, a workgroup
+// Three launches: δ (with lse beside it, the rows of a group side by side); d_q, a workgroup a tile of rows that walks the keys; d_k and d_v, a workgroup
 // a tile of keys that walks the rows of all of its group's heads. So every gradient
 // is summed by one workgroup in a fixed order, without atomics, and a group's shared
 // heads need no sum of their own; the price is that S and dP are formed twice (seven
@@ -27,11 +26,12 @@ struct BwdArgs {
   const void *q, *k, *v, *out, *d_out;
   const float* lse;
   void *d_q, *d_k, *d_v;
-  float2* stats;  // [kv_heads][tokens · G]: lse · log2(e), δ
+  float2* stats;  // [kv_heads][tokens · G]: −lse / scale, −δ: where S and dP start
   Spans spans;
   Group group;
   int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int kv_heads, dim, causal, tiles;
+  bool words;  // all operands lie in whole words
   float c, scale;
 };
 
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kNT) void attention_stats_kernel(BwdArgs p) {
   for (int w = 8; w; w >>= 1) t += __shfl_xor(t, w);
   if (lane == 0)
     p.stats[(int64_t(kv) * p.spans.tokens + token) * p.group.size + (hd - kv * p.group.size)] =
-        make_float2(p.lse[row] * kLog2E, t);
+        make_float2(-p.lse[row] * kLog2E / p.c, -t);
 }
 
 template <class T, int HD>
@@ -65,6 +65,7 @@ struct BwdShape {
   static constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // rows of a tile that is walked
   static constexpr int kBM = 4 * Mma<T>::kE;            // rows, or keys, of a workgroup
   static constexpr int kTileWords = kBN * Tile<T, HD>::kWords;
+  static constexpr bool kApart = sizeof(T) == 2 && HD >= 128;  // d_k and d_v
 };
 
 // A lane's row of a gradient: blocks of sums, a column of them the lane's own.
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
   using S = BwdShape<T, HD>;
   using Acc = typename M::Acc;
   constexpr int E = M::kE, BN = S::kBN, KB = BN / E, DB = HD / E, KS = HD / 16;
-  __shared__ uint4 smem[4 * S::kTileWords];
+  __shared__ uint4 smem[4 * S::kTileWords];  // keys, values; of two tiles
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % E, h = lane / E;
   const int G = p.group.size;
   const int head = int(blockIdx.x) % p.kv_heads;
@@ -118,10 +119,25 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
   const bool active = r0 + wave * E < rows;
   const int token = p.group.token(rc), hd = head * G + (rc - token * G);
   const int last = p.causal ? min(seq.keys - 1, token) : seq.keys - 1;
-  const Rows<T> ks{static_cast<const T*>(p.k) + int64_t(seq.k0) * p.ldk + int64_t(head) * p.dim,
-                   p.ldk, p.dim, Group{1, 0, 0}};
-  const Rows<T> vs{static_cast<const T*>(p.v) + int64_t(seq.k0) * p.ldv + int64_t(head) * p.dim,
-                   p.ldv, p.dim, Group{1, 0, 0}};
+  const Feed<T, HD, BN> keys(
+      Rows<T>{static_cast<const T*>(p.k) + int64_t(seq.k0) * p.ldk + int64_t(head) * p.dim, p.ldk,
+              p.dim, Group{1, 0, 0}},
+      p.words);
+  const Feed<T, HD, BN> values(
+      Rows<T>{static_cast<const T*>(p.v) + int64_t(seq.k0) * p.ldv + int64_t(head) * p.dim, p.ldv,
+              p.dim, Group{1, 0, 0}},
+      p.words);
+  const Reader<T, HD> read(lane);
+  auto load = [&](int n, int buf) {
+    const int there = min(BN, seq.keys - n * BN);
+    keys.load(smem + buf * 2 * S::kTileWords, n * BN, there);
+    values.load(smem + (buf * 2 + 1) * S::kTileWords, n * BN, there);
+  };
+  if (count > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keys.clear_rest(smem + i * S::kTileWords);
+    load(0, 0);
+  }
   uint4 q[KS], d[KS];
   {
     const T* qr = static_cast<const T*>(p.q) + int64_t(seq.q0 + token) * p.ldq + int64_t(hd) * p.dim;
@@ -134,91 +150,107 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
     }
   }
   const float2 stat = p.stats[(int64_t(head) * p.spans.tokens + seq.q0) * G + rc];
+  const float lse = stat.x * p.c, delta = stat.y;  // negative
   Acc dq[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int i = 0; i < M::kAcc; ++i) dq[b][i] = 0.f;
+  feed_barrier();
 
-  Stage<T, HD, BN, kNT> sk, sv;
-  auto tile_k = [&](int n) { return smem + (n & 1) * 2 * S::kTileWords; };
-  auto tile_v = [&](int n) { return tile_k(n) + S::kTileWords; };
-  auto partly = [&](int n) { return p.causal && (n + 1) * BN > all; };
-  int wild = 0;
-  if (count > 0) {
-    const int there = min(BN, seq.keys);
-    sk.load(ks, 0, there);
-    sv.load(vs, 0, there);
-    sk.store(tile_k(0), there);
-    sv.store(tile_v(0), there);
-    if (partly(0)) wild = __syncthreads_or(sk.wild(there));
-    else __syncthreads();
-  }
-  for (int n = 0; n < count; ++n) {
-    const int there = min(BN, seq.keys - (n + 1) * BN);
-    if (n + 1 < count) {
-      sk.load(ks, (n + 1) * BN, there);
-      sv.load(vs, (n + 1) * BN, there);
-    }
-    const uint4 *tk = tile_k(n), *tv = tile_v(n);
-    Acc x[KB];
+  auto step = [&](auto parity, auto partly, int n) {
+    constexpr int buf = decltype(parity)::value;
+    constexpr bool kPartly = decltype(partly)::value;
+    uint4* const key_tile = smem + buf * 2 * S::kTileWords;
+    const char* const tk = reinterpret_cast<const char*>(key_tile);
+    const char* const tv = reinterpret_cast<const char*>(key_tile + S::kTileWords);
+    if (n + 1 < count) load(n + 1, buf ^ 1);
+    static_assert(KB == 2, "a block's exponentials stand beside the other's products");
+    uint4 x[BN / 16];  // dS
+    Acc s[KB], g[KB];
+    auto scores = [&](auto block, auto beside) {
+      constexpr int b = decltype(block)::value;
+#pragma unroll
+      for (int i = 0; i < M::kAcc; ++i) s[b][i] = g[b][i] = 0.f;
+      in_turn<2 * KS, 3>(
+          [&](auto i) { return read.rows(i % 2 ? tv : tk, b, i / 2); },
+          [&](auto i, const uint4& w) {
+            constexpr int at = decltype(i)::value;
+            if constexpr (at % 2) M::mul(w, d[at / 2], g[b]);
+            else M::mul(w, q[at / 2], s[b]);
+            beside(i);
+          });
+    };
+    auto weigh = [&](int b, int i) {
+      float v = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, lse)) * (g[b][i] + delta);
+      if constexpr (kPartly) v = n * BN + b * E + M::row(i, h) <= last ? v : 0.f;
+      s[b][i] = v;
+    };
+    auto pack = [&](int b) {
+#pragma unroll
+      for (int u = 0; u < M::kHalves; ++u) x[b * M::kHalves + u] = M::operand(s[b], u);
+    };
+    constexpr int kProducts = M::kHalves * DB;
+    auto gradient = [&](auto block, auto beside) {
+      constexpr int b = decltype(block)::value;
+      in_turn<kProducts, 3>(
+          [&](auto i) { return read.cols(tk, i % DB, b * M::kHalves + i / DB); },
+          [&](auto i, const uint4& w) {
+            constexpr int at = decltype(i)::value;
+            M::mul(w, x[b * M::kHalves + at / DB], dq[at % DB]);
+            beside(i);
+          });
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    const auto nothing = [](auto) {};
     if (active) {
+      scores(B0{}, nothing);
+      scores(B1{}, [&](auto i) {
+        share<M::kAcc, 2 * KS, decltype(i)::value>([&](int e) { weigh(0, e); });
+      });
+      pack(0);
+      if constexpr (kPartly) {
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        Acc s, g;
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i) s[i] = g[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          M::mul(Tile<T, HD>::rows(tk, b, k, c, h), q[k], s);
-          M::mul(Tile<T, HD>::rows(tv, b, k, c, h), d[k], g);
-        }
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i)
-          x[b][i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -stat.x)) * (g[i] - stat.y);
-        if ((n + 1) * BN > all) {
-#pragma unroll
-          for (int i = 0; i < M::kAcc; ++i)
-            x[b][i] = n * BN + b * E + M::row(i, h) <= last ? x[b][i] : 0.f;
-        }
+        for (int i = 0; i < M::kAcc; ++i) weigh(1, i);
       }
     }
-    if (wild)  // whole workgroups, after the keys' own products
-      set_apart<T, HD, BN, kNT, DB>(tile_k(n), dq, h, [&](int j) { return n * BN + j <= last; });
-    if (active)
-      gemm::each<BN / 16>([&](auto step) {
-        constexpr int st = decltype(step)::value;
-        const uint4 w = M::template operand<st>(x);
-#pragma unroll
-        for (int b = 0; b < DB; ++b) M::mul(Tile<T, HD>::cols(tk, b, st, lane), w, dq[b]);
-      });
-    if (n + 1 < count) {
-      sk.store(tile_k(n + 1), there);
-      sv.store(tile_v(n + 1), there);
-      if (partly(n + 1)) wild = __syncthreads_or(sk.wild(there));
-      else __syncthreads();
+    if constexpr (kPartly) {
+      if (__syncthreads_or(Feed<T, HD, BN>::wild(key_tile)))
+        set_apart<T, HD, BN, kNT, DB>(key_tile, dq, h, [&](int j) { return n * BN + j <= last; });
     }
-  }
+    if (active) {
+      gradient(B0{}, [&](auto i) {
+        if constexpr (!kPartly)
+          share<M::kAcc, kProducts, decltype(i)::value>([&](int e) { weigh(1, e); });
+      });
+      pack(1);
+      gradient(B1{}, nothing);
+    }
+    feed_barrier();
+  };
+  walk(all / BN, count, step);
   if (r < rows)
     store_row<T, DB>(static_cast<T*>(p.d_q) + int64_t(seq.q0 + token) * p.lddq +
                          int64_t(hd) * p.dim, dq, p.scale, p.dim, h);
 }
 
-// d_k (DK) and d_v (DV) of a tile of keys. At 256 values a head the sums and operands
-// of both do not fit in registers, and they are launches of their own.
+// d_k (DK) and d_v (DV) of a tile of keys. In bf16 from 65 values a head on their sums and
+// operands together are more than the 256 registers of a lane with which a SIMD has two
+// waves, so they are apart, with S formed for each: one wave hands out an instruction
+// every five to eight cycles, too few to keep its matrix unit busy (8192 tokens in four
+// sequences, 16 heads on 4 of 128: 607 us apart, 745 together by one wave).
 template <class T, int HD, bool DK, bool DV>
-__global__ __launch_bounds__(kNT, 1) void attention_dkv_kernel(BwdArgs p) {
+__device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats, int block) {
   using M = Mma<T>;
   using S = BwdShape<T, HD>;
   using Acc = typename M::Acc;
   constexpr int E = M::kE, BN = S::kBN, KB = BN / E, DB = HD / E, KS = HD / 16;
-  __shared__ uint4 smem[4 * S::kTileWords];
-  __shared__ float2 stats[2 * BN];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % E, h = lane / E;
   const int G = p.group.size;
-  const int head = int(blockIdx.x) % p.kv_heads;
+  const int head = block % p.kv_heads;
   Seq seq;
-  if (!find_tile(p.spans, int(blockIdx.x) / p.kv_heads, 1, S::kBM, &seq)) return;
+  if (!find_tile(p.spans, block / p.kv_heads, 1, S::kBM, &seq)) return;
   const int rows = seq.keys ? seq.len * G : 0, j0 = seq.tile * S::kBM;
   const int j = j0 + wave * E + c, jc = min(j, seq.len - 1);
   const bool active = j0 + wave * E < seq.len;
@@ -226,10 +258,15 @@ __global__ __launch_bounds__(kNT, 1) void attention_dkv_kernel(BwdArgs p) {
   const int first = p.causal ? jc * G : 0;
   const int whole = p.causal ? min(seq.len, j0 + S::kBM) * G - G : 0;
   const int b0 = p.causal ? j0 * G / BN : 0, count = (rows + BN - 1) / BN;
-  const Rows<T> qs{static_cast<const T*>(p.q) + int64_t(seq.q0) * p.ldq +
-                       int64_t(head) * G * p.dim, p.ldq, p.dim, p.group};
-  const Rows<T> ds{static_cast<const T*>(p.d_out) + int64_t(seq.q0) * p.lddo +
-                       int64_t(head) * G * p.dim, p.lddo, p.dim, p.group};
+  const Feed<T, HD, BN> queries(
+      Rows<T>{static_cast<const T*>(p.q) + int64_t(seq.q0) * p.ldq + int64_t(head) * G * p.dim,
+              p.ldq, p.dim, p.group},
+      p.words);
+  const Feed<T, HD, BN> cotangents(
+      Rows<T>{static_cast<const T*>(p.d_out) + int64_t(seq.q0) * p.lddo +
+                  int64_t(head) * G * p.dim,
+              p.lddo, p.dim, p.group},
+      p.words);
   const float2* st = p.stats + (int64_t(head) * p.spans.tokens + seq.q0) * G;
   uint4 k[KS], v[DK ? KS : 1];
   {
@@ -243,87 +280,148 @@ __global__ __launch_bounds__(kNT, 1) void attention_dkv_kernel(BwdArgs p) {
   }
   Acc dk[DK ? DB : 1], dv[DV ? DB : 1];
 #pragma unroll
-  for (int i = 0; i < M::kAcc; ++i) {
+  for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int b = 0; b < DB; ++b) {
+    for (int i = 0; i < M::kAcc; ++i) {
       if constexpr (DK) dk[b][i] = 0.f;
       if constexpr (DV) dv[b][i] = 0.f;
     }
-  }
-  Stage<T, HD, BN, kNT> sq, sd;
+  const Reader<T, HD> read(lane);
   float2 ss;
-  auto tile_q = [&](int n) { return smem + (n & 1) * 2 * S::kTileWords; };
-  auto tile_d = [&](int n) { return tile_q(n) + S::kTileWords; };
-  auto partly = [&](int n) { return p.causal && n * BN < whole; };
-  int wild = 0;
-  auto load = [&](int n) {
+  auto load = [&](int n, int buf) {
     const int there = min(BN, rows - n * BN);
-    sq.load(qs, n * BN, there);
-    sd.load(ds, n * BN, there);
-    // Rows that are not there: weights of zero.
-    ss = make_float2(INFINITY, 0.f);
+    // Before the copies: what is written to a register in flight waits for all of them.
+    // Rows that are not there have weights of zero.
+    ss = make_float2(-INFINITY, 0.f);
     if (int(threadIdx.x) < there) ss = st[n * BN + threadIdx.x];
+    queries.load(smem + buf * 2 * S::kTileWords, n * BN, there);
+    cotangents.load(smem + (buf * 2 + 1) * S::kTileWords, n * BN, there);
   };
-  auto store = [&](int n) {
-    const int there = min(BN, rows - n * BN);
-    sq.store(tile_q(n), there);
-    sd.store(tile_d(n), there);
-    if (threadIdx.x < BN) stats[(n & 1) * BN + threadIdx.x] = ss;
-    wild = 0;
-    if (partly(n)) wild = __syncthreads_or((DK ? sq.wild(there) : 0) | (DV ? sd.wild(there) : 0));
-    else __syncthreads();
+  auto keep_stats = [&](int buf) {
+    if (threadIdx.x < BN) {
+      stats[buf * 2 * BN + threadIdx.x] = ss.x;
+      stats[(buf * 2 + 1) * BN + threadIdx.x] = ss.y;
+    }
   };
   if (b0 < count) {
-    load(b0);
-    store(b0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) queries.clear_rest(smem + i * S::kTileWords);
+    load(count - 1, 0);
+    keep_stats(0);
   }
-  for (int n = b0; n < count; ++n) {
-    if (n + 1 < count) load(n + 1);
-    const uint4 *tq = tile_q(n), *td = tile_d(n);
-    const float2* sn = stats + (n & 1) * BN;
-    Acc pr[KB], x[KB];
-    if (active) {
+  feed_barrier();
+  // From the last rows on: all workgroups of a head then read the same rows at the same
+  // time, which meet in L2.
+  auto step = [&](auto parity, auto partly, int n) {
+    constexpr int buf = decltype(parity)::value;
+    constexpr bool kPartly = decltype(partly)::value;
+    uint4* const query_tile = smem + buf * 2 * S::kTileWords;
+    const char* const tq = reinterpret_cast<const char*>(query_tile);
+    const char* const td = reinterpret_cast<const char*>(query_tile + S::kTileWords);
+    const float *start_s = stats + buf * 2 * BN, *start_g = start_s + BN;
+    if (n > b0) load(n - 1, buf ^ 1);
+    static_assert(KB == 2, "a block's exponentials stand beside the other's products");
+    constexpr int kTerms = (DK ? 2 : 1) * KS, kAhead = DK && sizeof(T) == 2 && HD == 128 ? 1 : 3;
+    uint4 x[DK ? BN / 16 : 1], w[DV ? BN / 16 : 1];  // dS, P
+    Acc s[KB], g[KB];
+    auto scores = [&](auto block, auto beside) {
+      constexpr int b = decltype(block)::value;
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        Acc s, g;
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i) s[i] = g[i] = 0.f;
-#pragma unroll
-        for (int u = 0; u < KS; ++u) {
-          M::mul(Tile<T, HD>::rows(tq, b, u, c, h), k[u], s);
-          if constexpr (DK) M::mul(Tile<T, HD>::rows(td, b, u, c, h), v[u], g);
-        }
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i) {
-          const float2 rs = sn[b * E + M::row(i, h)];
-          const float w = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -rs.x));
-          const bool on = !partly(n) || n * BN + b * E + M::row(i, h) >= first;
-          pr[b][i] = on ? w : 0.f;
-          if constexpr (DK) x[b][i] = on ? w * (g[i] - rs.y) : 0.f;
+      for (int i = 0; i < M::kAcc; i += 4) {
+        const float4 ls = *reinterpret_cast<const float4*>(start_s + b * E + M::row(i, h));
+        s[b][i] = ls.x;
+        s[b][i + 1] = ls.y;
+        s[b][i + 2] = ls.z;
+        s[b][i + 3] = ls.w;
+        if constexpr (DK) {
+          const float4 de = *reinterpret_cast<const float4*>(start_g + b * E + M::row(i, h));
+          g[b][i] = de.x;
+          g[b][i + 1] = de.y;
+          g[b][i + 2] = de.z;
+          g[b][i + 3] = de.w;
         }
       }
-    }
-    if (wild) {  // whole workgroups
-      const auto sees = [&](int i) { return n * BN + i >= first; };
-      if constexpr (DV) set_apart<T, HD, BN, kNT, DB>(tile_d(n), dv, h, sees);
-      if constexpr (DK) set_apart<T, HD, BN, kNT, DB>(tile_q(n), dk, h, sees);
-    }
-    if (active)
-      gemm::each<BN / 16>([&](auto step) {
-        constexpr int u = decltype(step)::value;
-        if constexpr (DV) {
-          const uint4 w = M::template operand<u>(pr);
+      in_turn<kTerms, kAhead>(
+          [&](auto i) {
+            return DK ? read.rows(i % 2 ? td : tq, b, i / 2) : read.rows(tq, b, i);
+          },
+          [&](auto i, const uint4& w) {
+            constexpr int at = decltype(i)::value;
+            if constexpr (!DK) M::mul(w, k[at], s[b]);
+            else if constexpr (at % 2) M::mul(w, v[at / 2], g[b]);
+            else M::mul(w, k[at / 2], s[b]);
+            beside(i);
+          });
+    };
+    auto weigh = [&](int b, int i) {
+      const bool on = !kPartly || n * BN + b * E + M::row(i, h) >= first;
+      float t = __builtin_amdgcn_exp2f(s[b][i] * p.c);
+      if constexpr (DK) {
+        float u = on ? t * g[b][i] : 0.f;
+        g[b][i] = u;
+      }
+      t = on ? t : 0.f;
+      s[b][i] = t;
+    };
+    auto pack = [&](int b) {
 #pragma unroll
-          for (int b = 0; b < DB; ++b) M::mul(Tile<T, HD>::cols(td, b, u, lane), w, dv[b]);
-        }
-        if constexpr (DK) {
-          const uint4 w = M::template operand<u>(x);
-#pragma unroll
-          for (int b = 0; b < DB; ++b) M::mul(Tile<T, HD>::cols(tq, b, u, lane), w, dk[b]);
-        }
+      for (int u = 0; u < M::kHalves; ++u) {
+        if constexpr (DK) x[b * M::kHalves + u] = M::operand(g[b], u);
+        if constexpr (DV) w[b * M::kHalves + u] = M::operand(s[b], u);
+      }
+    };
+    constexpr int kBoth = DK + DV, kProducts = M::kHalves * DB * kBoth;
+    auto gradient = [&](auto block, auto beside) {
+      constexpr int b = decltype(block)::value;
+      in_turn<kProducts, kAhead>(
+          [&](auto i) {
+            constexpr int at = decltype(i)::value, u = at / kBoth;
+            return read.cols(DK && at % kBoth == 0 ? tq : td, u % DB, b * M::kHalves + u / DB);
+          },
+          [&](auto i, const uint4& a) {
+            constexpr int at = decltype(i)::value, u = at / kBoth;
+            if constexpr (DK && at % kBoth == 0) M::mul(a, x[b * M::kHalves + u / DB], dk[u % DB]);
+            else M::mul(a, w[b * M::kHalves + u / DB], dv[u % DB]);
+            beside(i);
+          });
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    const auto nothing = [](auto) {};
+    if (active) {
+      scores(B0{}, nothing);
+      scores(B1{}, [&](auto i) {
+        share<M::kAcc, kTerms, decltype(i)::value>([&](int e) { weigh(0, e); });
       });
-    if (n + 1 < count) store(n + 1);
-  }
+      pack(0);
+      if constexpr (kPartly) {
+#pragma unroll
+        for (int i = 0; i < M::kAcc; ++i) weigh(1, i);
+      }
+    }
+    if constexpr (kPartly) {
+      const int bad = (DK ? Feed<T, HD, BN>::wild(query_tile) : 0) |
+                      (DV ? Feed<T, HD, BN>::wild(query_tile + S::kTileWords) : 0);
+      if (__syncthreads_or(bad)) {
+        const auto sees = [&](int i) { return n * BN + i >= first; };
+        if constexpr (DK) set_apart<T, HD, BN, kNT, DB>(query_tile, dk, h, sees);
+        if constexpr (DV) set_apart<T, HD, BN, kNT, DB>(query_tile + S::kTileWords, dv, h, sees);
+      }
+    }
+    if (active) {
+      gradient(B0{}, [&](auto i) {
+        if constexpr (!kPartly)
+          share<M::kAcc, kProducts, decltype(i)::value>([&](int e) { weigh(1, e); });
+      });
+      pack(1);
+      gradient(B1{}, nothing);
+    }
+    if (n > b0) keep_stats(buf ^ 1);
+    feed_barrier();
+  };
+  // Tiles from `whole` on are seen whole.
+  walk(count - (p.causal ? (whole + BN - 1) / BN : 0), count - b0,
+       [&](auto parity, auto partly, int i) { step(parity, partly, count - 1 - i); });
   if (j >= seq.len) return;
   if constexpr (DK)
     store_row<T, DB>(static_cast<T*>(p.d_k) + int64_t(seq.q0 + j) * p.lddk +
@@ -332,16 +430,25 @@ __global__ __launch_bounds__(kNT, 1) void attention_dkv_kernel(BwdArgs p) {
     store_row<T, DB>(static_cast<T*>(p.d_v) + int64_t(seq.q0 + j) * p.lddv +
                          int64_t(head) * p.dim, dv, 1.f, p.dim, h);
 }
-
-template <class T, int HD, bool DK, bool DV>
-hipError_t dkv_go(BwdArgs p, hipStream_t stream) {
+// One of them may be left out; where they are apart, d_k's workgroups (`first_v` of them)
+// come before d_v's.
+template <class T, int HD>
+__global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dkv_kernel(
+    BwdArgs p, int first_v) {
   using S = BwdShape<T, HD>;
-  const auto fn = attention_dkv_kernel<T, HD, DK, DV>;
-  p.tiles = int(tile_count(p.spans.tokens, 1, S::kBM, p.spans.sequences));
-  ProfScope ps("dn_attention_dkv", stream);
-  hipLaunchKernelGGL(fn, dim3(unsigned(p.tiles) * unsigned(p.kv_heads)), dim3(kNT), 0,
-                     stream, p);
-  return hipGetLastError();
+  __shared__ uint4 smem[4 * S::kTileWords];  // queries, d_out; of two tiles
+  __shared__ __attribute__((aligned(16))) float stats[4 * S::kBN];
+  const int block = int(blockIdx.x);
+  if constexpr (S::kApart) {
+    if (block < first_v) key_gradients<T, HD, true, false>(p, smem, stats, block);
+    else key_gradients<T, HD, false, true>(p, smem, stats, block - first_v);
+  } else if (!p.d_v) {
+    key_gradients<T, HD, true, false>(p, smem, stats, block);
+  } else if (!p.d_k) {
+    key_gradients<T, HD, false, true>(p, smem, stats, block);
+  } else {
+    key_gradients<T, HD, true, true>(p, smem, stats, block);
+  }
 }
 
 template <class T, int HD>
@@ -364,11 +471,14 @@ hipError_t bwd_go(const BwdArgs& a, hipStream_t stream) {
                        stream, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  if constexpr (HD <= 128) {
-    if (p.d_k && p.d_v) return dkv_go<T, HD, true, true>(p, stream);
-  }
-  if (p.d_k && (e = dkv_go<T, HD, true, false>(p, stream)) != hipSuccess) return e;
-  return p.d_v ? dkv_go<T, HD, false, true>(p, stream) : hipSuccess;
+  if (!p.d_k && !p.d_v) return hipSuccess;
+  p.tiles = int(tile_count(p.spans.tokens, 1, S::kBM, p.spans.sequences));
+  const int blocks = p.tiles * p.kv_heads;
+  ProfScope ps("dn_attention_dkv", stream);
+  const int groups = S::kApart && p.d_k && p.d_v ? 2 * blocks : blocks;
+  hipLaunchKernelGGL((attention_dkv_kernel<T, HD>), dim3(unsigned(groups)), dim3(kNT), 0, stream, p,
+                     p.d_k ? blocks : 0);
+  return hipGetLastError();
 }
 template <class T>
 hipError_t bwd_typed(const BwdArgs& p, hipStream_t stream) {
@@ -412,6 +522,7 @@ hipError_t launch_attention_bwd(const dn_attention_bwd_args& a, float scale, voi
   p.causal = a.causal;
   p.c = scale * kLog2E;
   p.scale = scale;
+  p.words = in_words(a.dtype, p.dim, {{a.q, p.ldq}, {a.k, p.ldk}, {a.v, p.ldv}, {a.d_out, p.lddo}});
   return a.dtype == DN_BF16 ? bwd_typed<bf16>(p, stream) : bwd_typed<float>(p, stream);
 }
 
