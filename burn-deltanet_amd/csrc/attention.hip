@@ -220,13 +220,14 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
   if (p.lse && h == 0) p.lse[at] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) / kLog2E;
 }
 
-// The parts of a row: a wave a row, 64 columns at a time.
+// The parts of a row: a workgroup a row, its waves taking every fourth part, two columns a
+// lane; their sums meet in LDS.
+constexpr int kMostSplits = 256;
 template <class T>
 __global__ __launch_bounds__(kNT) void attention_join_kernel(FwdArgs p) {
-  const int heads = p.group.size * p.kv_heads, lane = threadIdx.x & 63;
-  const int64_t rows = int64_t(p.spans.tokens) * heads;
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  __shared__ float weight[kMostSplits], part[4][128];
+  const int heads = p.group.size * p.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t rows = int64_t(p.spans.tokens) * heads, row = blockIdx.x;
   float top = -INFINITY;
   for (int s = lane; s < p.splits; s += 64) top = fmaxf(top, p.part_ml[s * rows + row].x);
 #pragma unroll
@@ -235,23 +236,41 @@ __global__ __launch_bounds__(kNT) void attention_join_kernel(FwdArgs p) {
   float sum = 0.f;
   for (int s = lane; s < p.splits; s += 64) {
     const float2 ml = p.part_ml[s * rows + row];
-    sum += ml.y * __builtin_amdgcn_exp2f(ml.x - base);
+    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+    sum += ml.y * f;
+    if (wave == 0) weight[s] = f;
   }
 #pragma unroll
   for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
+  __syncthreads();
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int64_t token = row / heads;
   T* out = static_cast<T*>(p.out) + token * p.ldo + (row - token * heads) * p.dim;
-  for (int col = lane; col < p.dim; col += 64) {
-    float v = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const float f = __builtin_amdgcn_exp2f(p.part_ml[s * rows + row].x - base);
-      v += p.part[(s * rows + row) * p.dim + col] * f;
+  for (int c0 = 0; c0 < p.dim; c0 += 128) {
+    const int col = c0 + 2 * lane;
+    float2 v = make_float2(0.f, 0.f);
+    if (col + 1 < p.dim) {
+#pragma unroll 8
+      for (int s = wave; s < p.splits; s += 4) {
+        float2 x;
+        __builtin_memcpy(&x, p.part + (s * rows + row) * p.dim + col, 8);
+        v.x = fmaf(x.x, weight[s], v.x);
+        v.y = fmaf(x.y, weight[s], v.y);
+      }
+    } else if (col < p.dim) {
+      for (int s = wave; s < p.splits; s += 4)
+        v.x = fmaf(p.part[(s * rows + row) * p.dim + col], weight[s], v.x);
     }
-    st(out, size_t(col), v * inv);
+    part[wave][2 * lane] = v.x;
+    part[wave][2 * lane + 1] = v.y;
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < 128 && c0 + c < p.dim)
+      st(out, size_t(c0 + c), (part[0][c] + part[1][c] + part[2][c] + part[3][c]) * inv);
+    __syncthreads();
   }
-  if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) / kLog2E;
+  if (p.lse && threadIdx.x == 0)
+    p.lse[row] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) / kLog2E;
 }
 
 int padded_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -259,8 +278,10 @@ int64_t tile_rows(int dtype) {
   return 4 * (dtype == DN_BF16 ? Mma<bf16>::kE : Mma<float>::kE);
 }
 
-// Parts of the keys: none where the tiles of rows fill the CUs twice, else as many as
-// do, of at least 256 keys each on average.
+// Parts of the keys, of at least 256 keys each on average: as many as fill the CUs twice
+// where the tiles of rows do not. (More, to even out sequences of different lengths, gain
+// nothing: 64 requests of a token over 2048 to 8192 keys, 16 heads on 4 of 128, 183 us
+// with twice the CUs' workgroups and 186 with eight times.)
 int splits_of(const dn_attention_args& a) {
   const int64_t group = a.nheads / a.kv_heads;
   const int64_t tiles =
@@ -268,7 +289,7 @@ int splits_of(const dn_attention_args& a) {
   const int64_t want = 2 * device_cu_count() / std::max<int64_t>(1, tiles);
   const int64_t keys = a.key_starts ? a.key_rows : a.tokens;
   const int64_t most = keys / std::max<int64_t>(1, a.sequences) / 256;
-  return int(std::max<int64_t>(1, std::min<int64_t>({want, most, 256})));
+  return int(std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits})));
 }
 
 template <class T, int HD>
@@ -283,8 +304,7 @@ hipError_t fwd_go(const FwdArgs& p, hipStream_t stream) {
   if (e != hipSuccess || !p.part) return e;
   ProfScope ps("dn_attention_join", stream);
   const int64_t rows = int64_t(p.spans.tokens) * p.group.size * p.kv_heads;
-  hipLaunchKernelGGL((attention_join_kernel<T>), dim3(unsigned((rows + 3) / 4)), dim3(kNT), 0,
-                     stream, p);
+  hipLaunchKernelGGL((attention_join_kernel<T>), dim3(unsigned(rows)), dim3(kNT), 0, stream, p);
   return hipGetLastError();
 }
 template <class T>

@@ -12,10 +12,10 @@
 //     share of the tokens, an id at a time, what belongs to the range and what lies
 //     below it, which is where the range's tokens start in the sorted order; then
 //     each wave puts down its tokens where its counts say, so that an id's tokens
-//     stand in their order. The range's rows that no token names are zeroed here.
+//     stand in their order.
 //  2. Sums of 32 consecutive sorted tokens each, however few or many share an id: a run
 //     that lies inside is written, one that crosses an end leaves its part in the
-//     workspace (fp32).
+//     workspace (fp32). Further workgroups write the rows that no token names.
 //  3. The parts of the runs that cross, in order.
 #include <algorithm>
 
@@ -64,23 +64,22 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(const ID* ids, cons
 }
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kIdsAhead = 8;  // steps of 64 tokens whose ids a wave has in flight
 
 struct SortArgs {
   const void* ids;
-  void* d_table;
   int *pos, *key, *total;  // sorted: the token and its id; how many there are
-  int64_t ldt;
-  int tokens, vocab, dim, width;  // width: ids of a workgroup
+  int* count;              // [vocab] tokens of each id
+  int tokens, vocab, width;  // width: ids of a workgroup
 };
 
-template <class T, class ID>
+template <class ID>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs p) {
-  extern __shared__ int counts[];  // [waves][width], then [width] of all waves
+  extern __shared__ int counts[];  // [waves][width]
   __shared__ int scan[kSortThreads], below[kSortWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, width = p.width;
   const int lo = int(blockIdx.x) * width, n = min(width, p.vocab - lo);
   const ID* ids = static_cast<const ID*>(p.ids);
-  int* totals = counts + kSortWaves * width;
   for (int i = threadIdx.x; i < kSortWaves * width; i += kSortThreads) counts[i] = 0;
   __syncthreads();
   // A wave's share of the tokens: whole steps of 64.
@@ -88,10 +87,19 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs p
   const int64_t first = int64_t(wave) * share, end = min(first + share, int64_t(p.tokens));
   int* mine = counts + wave * width;
   int less = 0;
-  for (int64_t i = first + lane; i < end; i += 64) {
-    const int64_t id = int64_t(ids[i]);
-    if (id >= 0 && id < lo) ++less;
-    if (id >= lo && id < lo + n) atomicAdd(&mine[int(id - lo)], 1);
+  for (int64_t i0 = first; i0 < end; i0 += 64 * kIdsAhead) {
+    ID next[kIdsAhead];
+#pragma unroll
+    for (int j = 0; j < kIdsAhead; ++j) {
+      const int64_t i = i0 + 64 * j + lane;
+      next[j] = i < end ? ids[i] : ID(-1);
+    }
+#pragma unroll
+    for (int j = 0; j < kIdsAhead; ++j) {
+      const int64_t id = int64_t(next[j]);
+      if (id >= 0 && id < lo) ++less;
+      if (id >= lo && id < lo + n) atomicAdd(&mine[int(id - lo)], 1);
+    }
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) less += __shfl_xor(less, o);
@@ -120,53 +128,75 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs p
     if (i < n) {
       const int start = base + scan[threadIdx.x] - t;
       for (int w = 0; w < kSortWaves; ++w) counts[w * width + i] += start;
-      totals[i] = t;
+      p.count[lo + i] = t;
     }
     base += scan[kSortThreads - 1];
     __syncthreads();
   }
   if (blockIdx.x + 1 == gridDim.x && threadIdx.x == 0) *p.total = base;
-  // Tokens of one id within a step stand in the order of their lanes.
-  for (int64_t i0 = first; i0 < end; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const int64_t id = i < end ? int64_t(ids[i]) : -1;
-    const bool in = id >= lo && id < lo + n;
-    uint64_t left = __ballot(in);
-    while (left) {
-      const int leader = int(__ffsll(static_cast<unsigned long long>(left))) - 1;
-      const int key = __builtin_amdgcn_readlane(int(id - lo), leader);
-      const uint64_t same = __ballot(in && int(id - lo) == key);
-      if (in && int(id - lo) == key) {
-        const int at = mine[key] + int(__popcll(same & ((uint64_t(1) << lane) - 1)));
-        p.pos[at] = int(i);
-        p.key[at] = lo + key;
-      }
-      if (lane == leader) mine[key] += int(__popcll(same));
-      left &= ~same;
+  // Tokens of one id within a step stand in the order of their lanes. Lanes of one id find
+  // each other by the bits of their ids (one ballot a bit: a loop over the ids of a step
+  // took 81 us in place of 18 for 16384 tokens as text has them, half of whom one range
+  // holds).
+  int bits = 0;
+  while ((1 << bits) < n) ++bits;
+  for (int64_t i0 = first; i0 < end; i0 += 64 * kIdsAhead) {
+    ID next[kIdsAhead];
+#pragma unroll
+    for (int j = 0; j < kIdsAhead; ++j) {
+      const int64_t i = i0 + 64 * j + lane;
+      next[j] = i < end ? ids[i] : ID(-1);
     }
-  }
-  // Rows of ids that no token has.
-  T* table = static_cast<T*>(p.d_table);
-  const float zero[8] = {};
-  for (int i = wave; i < n; i += kSortWaves) {
-    if (totals[i]) continue;
-    T* row = table + int64_t(lo + i) * p.ldt;
-    for (int col = lane * 8; col < p.dim; col += 512) store8(row + col, zero, p.dim - col);
+#pragma unroll
+    for (int j = 0; j < kIdsAhead; ++j) {
+      const int64_t id = int64_t(next[j]);
+      const bool in = id >= lo && id < lo + n;
+      uint64_t same = __ballot(in);
+      if (!same) continue;
+      const int key = in ? int(id - lo) : 0;
+      for (int b = 0; b < bits; ++b) {
+        const bool set = key >> b & 1;
+        const uint64_t all = __ballot(set);
+        same &= set ? all : ~all;
+      }
+      if (in) {
+        const int rank = int(__popcll(same & ((uint64_t(1) << lane) - 1)));
+        const int at = mine[key] + rank;
+        p.pos[at] = int(i0 + 64 * j + lane);
+        p.key[at] = lo + key;
+        if (rank == 0) mine[key] = at + int(__popcll(same));
+      }
+    }
   }
 }
 
 struct SumArgs {
   const void* d_out;
   void* d_table;
-  const int *pos, *key, *total;
+  const int *pos, *key, *total, *count;
+  int64_t groups;  // of workgroups that sum; the others write zeros
+  int vocab;
   float* part;  // [runs][2][dim]: what a run of tokens leaves at its start, at its end
   int64_t ldd, ldt;
   int dim, lanes;
   float scale;
 };
 
+constexpr int kZeroRows = 32;  // of a workgroup that writes zeros
+
 template <class T>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(SumArgs p) {
+  if (blockIdx.x >= p.groups) {  // rows of ids that no token has
+    const int64_t first = (blockIdx.x - p.groups) * kZeroRows;
+    const int rows = kThreads / p.lanes;
+    const int col = (threadIdx.x % p.lanes + int(blockIdx.y) * p.lanes) * 8, valid = p.dim - col;
+    const float zero[8] = {};
+    if (valid <= 0) return;
+    for (int64_t r = first + threadIdx.x / p.lanes; r < min(first + kZeroRows, int64_t(p.vocab));
+         r += rows)
+      if (!p.count[r]) store8(static_cast<T*>(p.d_table) + r * p.ldt + col, zero, valid);
+    return;
+  }
   const int64_t run = int64_t(blockIdx.x) * (kThreads / p.lanes) + threadIdx.x / p.lanes;
   const int total = *p.total;
   const int64_t p0 = run * kRun;
@@ -251,14 +281,14 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(SumArgs p) {
 }
 
 // Ids of a sorting workgroup: one for every CU, but no more than 512 ids each (their
-// counts by wave are 34 KB of LDS).
+// counts by wave are 32 KB of LDS).
 int sort_width(int64_t vocab) {
   const int64_t all = (vocab + device_cu_count() - 1) / device_cu_count();
   return int(std::max<int64_t>(1, std::min<int64_t>(all, 512)));
 }
 
 struct Layout {
-  size_t pos, key, total, part, bytes;
+  size_t pos, key, total, count, part, bytes;
 };
 Layout layout_of(const dn_embedding_bwd_args& a) {
   Layout l{};
@@ -266,7 +296,8 @@ Layout layout_of(const dn_embedding_bwd_args& a) {
   l.pos = 0;
   l.key = align_up(n * 4, 256);
   l.total = l.key + align_up(n * 4, 256);
-  l.part = l.total + 256;
+  l.count = l.total + 256;
+  l.part = l.count + align_up(size_t(a.vocab) * 4, 256);
   l.bytes = l.part + (runs > 1 ? runs * 2 * size_t(a.dim) * 4 : 0);
   return l;
 }
@@ -277,29 +308,29 @@ hipError_t bwd_go(const dn_embedding_bwd_args& a, void* ws, hipStream_t stream) 
   char* base = static_cast<char*>(ws);
   SortArgs s{};
   s.ids = a.ids;
-  s.d_table = a.d_table;
   s.pos = reinterpret_cast<int*>(base + l.pos);
   s.key = reinterpret_cast<int*>(base + l.key);
   s.total = reinterpret_cast<int*>(base + l.total);
-  s.ldt = a.d_table_stride;
+  s.count = reinterpret_cast<int*>(base + l.count);
   s.tokens = int(a.tokens);
   s.vocab = int(a.vocab);
-  s.dim = int(a.dim);
   s.width = sort_width(a.vocab);
   {
     ProfScope ps("dn_embedding_sort", stream);
-    hipLaunchKernelGGL((embedding_sort_kernel<T, ID>),
+    hipLaunchKernelGGL((embedding_sort_kernel<ID>),
                        dim3(unsigned((a.vocab + s.width - 1) / s.width)), dim3(kSortThreads),
-                       size_t(kSortWaves + 1) * size_t(s.width) * 4, stream, s);
+                       size_t(kSortWaves) * size_t(s.width) * 4, stream, s);
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.tokens == 0) return e;
+  if (e != hipSuccess) return e;
   SumArgs p{};
   p.d_out = a.d_out;
   p.d_table = a.d_table;
   p.pos = s.pos;
   p.key = s.key;
   p.total = s.total;
+  p.count = s.count;
+  p.vocab = s.vocab;
   p.part = reinterpret_cast<float*>(base + l.part);
   p.ldd = a.d_out_stride;
   p.ldt = a.d_table_stride;
@@ -307,15 +338,16 @@ hipError_t bwd_go(const dn_embedding_bwd_args& a, void* ws, hipStream_t stream) 
   p.lanes = lanes_of(a.dim);
   p.scale = float(a.scale);
   const int64_t runs = (a.tokens + kRun - 1) / kRun, at_once = kThreads / p.lanes;
+  p.groups = (runs + at_once - 1) / at_once;
   {
     ProfScope ps("dn_embedding_sum", stream);
     hipLaunchKernelGGL((embedding_sum_kernel<T>),
-                       dim3(unsigned((runs + at_once - 1) / at_once),
+                       dim3(unsigned(p.groups + (a.vocab + kZeroRows - 1) / kZeroRows),
                             unsigned((a.dim + p.lanes * 8 - 1) / (p.lanes * 8))),
                        dim3(kThreads), 0, stream, p);
   }
   e = hipGetLastError();
-  if (e != hipSuccess || runs == 1) return e;
+  if (e != hipSuccess || runs <= 1) return e;
   ProfScope ps("dn_embedding_join", stream);
   hipLaunchKernelGGL((embedding_join_kernel<T>),
                      dim3(unsigned(runs - 1), unsigned((a.dim + kJoinCols - 1) / kJoinCols)),
