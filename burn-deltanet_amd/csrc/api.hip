@@ -1209,7 +1209,8 @@ int check_block_norm_bwd(const dn_block_norm_bwd_args* a) {
 int check_embedding_sizes(int64_t tokens, int64_t vocab, int64_t dim, int32_t dtype, double scale) {
   if (tokens < 0) return fail(DN_ERR_SHAPE, "tokens must not be negative");
   if (int rc = check_sizes(tokens, {vocab, dim})) return rc;
-  if (tokens > (int64_t(1) << 28)) return fail(DN_ERR_SHAPE, "tensor too large");
+  if (tokens > (int64_t(1) << 28) || dim > (int64_t(1) << 23))
+    return fail(DN_ERR_SHAPE, "tensor too large");
   if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
   return std::isfinite(scale) ? DN_OK : fail(DN_ERR_SHAPE, "scale must be finite");
 }
@@ -1241,9 +1242,8 @@ int check_heads(int64_t tokens, int64_t sequences, int64_t nheads, int64_t kv_he
   if (nheads > 65536 || tokens > INT32_MAX / 2 || sequences > INT32_MAX / 2 ||
       (tokens + sequences) * nheads > INT32_MAX / 2)
     return fail(DN_ERR_SHAPE, "tensor too large");
-  // A launch has fewer than 2^32 threads: tiles of 64 rows at the least, two workgroups
-  // of 256 threads to a tile of keys.
-  if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 23))
+  // A launch has fewer than 2^32 threads: 16 to a row, or 256 to a tile of 64 rows.
+  if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 22))
     return fail(DN_ERR_SHAPE, "tensor too large");
   if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
   if (!std::isnan(scale) && !(scale > 0.0 && float(scale) > 0.f && std::isfinite(float(scale))))

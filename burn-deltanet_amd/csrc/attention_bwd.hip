@@ -10,8 +10,14 @@
 // products in place of five). Every product leaves its sums where the next one takes
 // them as an operand (attention.hpp).
 //
-// Sums are fp32; in bf16 the matrix unit takes P and dS rounded, the gradients are
-// rounded once.
+// Sums are fp32; in bf16 the matrix unit takes P and dS rounded (the gradients are 0.0025
+// from a 64-bit result in the norm, where rounding the result alone gives 0.0017), the
+// gradients are rounded once.
+//
+// Bound by the order in which a wave hands out its instructions: at 128 values a head two
+// waves a SIMD keep the matrix unit at half of its rate. Measured, one causal sequence of
+// 16384, 16 heads on 4 of 128, bf16: d_q 1.45 ms (1.1 PFLOP/s), d_k and d_v 2.7 ms (1.0
+// PFLOP/s with S formed twice), delta 26 us.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -65,7 +71,11 @@ struct BwdShape {
   static constexpr int kBN = sizeof(T) == 2 ? 64 : 32;  // rows of a tile that is walked
   static constexpr int kBM = 4 * Mma<T>::kE;            // rows, or keys, of a workgroup
   static constexpr int kTileWords = kBN * Tile<T, HD>::kWords;
-  static constexpr bool kApart = sizeof(T) == 2 && HD >= 128;  // d_k and d_v
+  static constexpr bool kApart = (sizeof(T) == 2 && HD == 128) || HD == 256;  // d_k and d_v
+  // For want of registers: one block of scores at a time; and the next tile's copies go
+  // behind them, as operands that come back from scratch memory wait for every copy
+  // issued before.
+  static constexpr bool kLarge = HD == 256;
 };
 
 // A lane's row of a gradient: blocks of sums, a column of them the lane's own.
@@ -164,7 +174,7 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
     uint4* const key_tile = smem + buf * 2 * S::kTileWords;
     const char* const tk = reinterpret_cast<const char*>(key_tile);
     const char* const tv = reinterpret_cast<const char*>(key_tile + S::kTileWords);
-    if (n + 1 < count) load(n + 1, buf ^ 1);
+    if (!S::kLarge && n + 1 < count) load(n + 1, buf ^ 1);
     static_assert(KB == 2, "a block's exponentials stand beside the other's products");
     uint4 x[BN / 16];  // dS
     Acc s[KB], g[KB];
@@ -186,6 +196,10 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
       if constexpr (kPartly) v = n * BN + b * E + M::row(i, h) <= last ? v : 0.f;
       s[b][i] = v;
     };
+    auto weigh_all = [&](int b) {
+#pragma unroll
+      for (int i = 0; i < M::kAcc; ++i) weigh(b, i);
+    };
     auto pack = [&](int b) {
 #pragma unroll
       for (int u = 0; u < M::kHalves; ++u) x[b * M::kHalves + u] = M::operand(s[b], u);
@@ -206,22 +220,22 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
     const auto nothing = [](auto) {};
     if (active) {
       scores(B0{}, nothing);
+      if constexpr (S::kLarge) weigh_all(0);
       scores(B1{}, [&](auto i) {
-        share<M::kAcc, 2 * KS, decltype(i)::value>([&](int e) { weigh(0, e); });
+        if constexpr (!S::kLarge)
+          share<M::kAcc, 2 * KS, decltype(i)::value>([&](int e) { weigh(0, e); });
       });
       pack(0);
-      if constexpr (kPartly) {
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i) weigh(1, i);
-      }
+      if constexpr (kPartly || S::kLarge) weigh_all(1);
     }
+    if (S::kLarge && n + 1 < count) load(n + 1, buf ^ 1);
     if constexpr (kPartly) {
       if (__syncthreads_or(Feed<T, HD, BN>::wild(key_tile)))
         set_apart<T, HD, BN, kNT, DB>(key_tile, dq, h, [&](int j) { return n * BN + j <= last; });
     }
     if (active) {
       gradient(B0{}, [&](auto i) {
-        if constexpr (!kPartly)
+        if constexpr (!kPartly && !S::kLarge)
           share<M::kAcc, kProducts, decltype(i)::value>([&](int e) { weigh(1, e); });
       });
       pack(1);
@@ -319,7 +333,7 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
     const char* const tq = reinterpret_cast<const char*>(query_tile);
     const char* const td = reinterpret_cast<const char*>(query_tile + S::kTileWords);
     const float *start_s = stats + buf * 2 * BN, *start_g = start_s + BN;
-    if (n > b0) load(n - 1, buf ^ 1);
+    if (!S::kLarge && n > b0) load(n - 1, buf ^ 1);
     static_assert(KB == 2, "a block's exponentials stand beside the other's products");
     constexpr int kTerms = (DK ? 2 : 1) * KS, kAhead = DK && sizeof(T) == 2 && HD == 128 ? 1 : 3;
     uint4 x[DK ? BN / 16 : 1], w[DV ? BN / 16 : 1];  // dS, P
@@ -363,6 +377,10 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
       t = on ? t : 0.f;
       s[b][i] = t;
     };
+    auto weigh_all = [&](int b) {
+#pragma unroll
+      for (int i = 0; i < M::kAcc; ++i) weigh(b, i);
+    };
     auto pack = [&](int b) {
 #pragma unroll
       for (int u = 0; u < M::kHalves; ++u) {
@@ -390,15 +408,15 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
     const auto nothing = [](auto) {};
     if (active) {
       scores(B0{}, nothing);
+      if constexpr (S::kLarge) weigh_all(0);
       scores(B1{}, [&](auto i) {
-        share<M::kAcc, kTerms, decltype(i)::value>([&](int e) { weigh(0, e); });
+        if constexpr (!S::kLarge)
+          share<M::kAcc, kTerms, decltype(i)::value>([&](int e) { weigh(0, e); });
       });
       pack(0);
-      if constexpr (kPartly) {
-#pragma unroll
-        for (int i = 0; i < M::kAcc; ++i) weigh(1, i);
-      }
+      if constexpr (kPartly || S::kLarge) weigh_all(1);
     }
+    if (S::kLarge && n > b0) load(n - 1, buf ^ 1);
     if constexpr (kPartly) {
       const int bad = (DK ? Feed<T, HD, BN>::wild(query_tile) : 0) |
                       (DV ? Feed<T, HD, BN>::wild(query_tile + S::kTileWords) : 0);
@@ -410,7 +428,7 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
     }
     if (active) {
       gradient(B0{}, [&](auto i) {
-        if constexpr (!kPartly)
+        if constexpr (!kPartly && !S::kLarge)
           share<M::kAcc, kProducts, decltype(i)::value>([&](int e) { weigh(1, e); });
       });
       pack(1);
@@ -430,8 +448,8 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
     store_row<T, DB>(static_cast<T*>(p.d_v) + int64_t(seq.q0 + j) * p.lddv +
                          int64_t(head) * p.dim, dv, 1.f, p.dim, h);
 }
-// One of them may be left out; where they are apart, d_k's workgroups (`first_v` of them)
-// come before d_v's.
+// Apart: d_k's workgroups (`first_v` of them) come before d_v's, and either may be left
+// out. Together: first_v is negative.
 template <class T, int HD>
 __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dkv_kernel(
     BwdArgs p, int first_v) {
@@ -439,16 +457,14 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dkv_kernel(
   __shared__ uint4 smem[4 * S::kTileWords];  // queries, d_out; of two tiles
   __shared__ __attribute__((aligned(16))) float stats[4 * S::kBN];
   const int block = int(blockIdx.x);
-  if constexpr (S::kApart) {
-    if (block < first_v) key_gradients<T, HD, true, false>(p, smem, stats, block);
-    else key_gradients<T, HD, false, true>(p, smem, stats, block - first_v);
-  } else if (!p.d_v) {
-    key_gradients<T, HD, true, false>(p, smem, stats, block);
-  } else if (!p.d_k) {
-    key_gradients<T, HD, false, true>(p, smem, stats, block);
-  } else {
-    key_gradients<T, HD, true, true>(p, smem, stats, block);
+  if constexpr (!S::kApart) {
+    if (first_v < 0) {
+      key_gradients<T, HD, true, true>(p, smem, stats, block);
+      return;
+    }
   }
+  if (block < first_v) key_gradients<T, HD, true, false>(p, smem, stats, block);
+  else key_gradients<T, HD, false, true>(p, smem, stats, block - first_v);
 }
 
 template <class T, int HD>
@@ -475,9 +491,10 @@ hipError_t bwd_go(const BwdArgs& a, hipStream_t stream) {
   p.tiles = int(tile_count(p.spans.tokens, 1, S::kBM, p.spans.sequences));
   const int blocks = p.tiles * p.kv_heads;
   ProfScope ps("dn_attention_dkv", stream);
-  const int groups = S::kApart && p.d_k && p.d_v ? 2 * blocks : blocks;
-  hipLaunchKernelGGL((attention_dkv_kernel<T, HD>), dim3(unsigned(groups)), dim3(kNT), 0, stream, p,
-                     p.d_k ? blocks : 0);
+  // Apart too where the tiles of keys are too few to fill the CUs twice.
+  const bool both = p.d_k && p.d_v, apart = S::kApart || blocks < 2 * device_cu_count();
+  hipLaunchKernelGGL((attention_dkv_kernel<T, HD>), dim3(unsigned(both && apart ? 2 * blocks : blocks)),
+                     dim3(kNT), 0, stream, p, both && !apart ? -1 : p.d_k ? blocks : 0);
   return hipGetLastError();
 }
 template <class T>

@@ -18,7 +18,11 @@
 // adds the workgroups' in order. Rows too long for registers are read again.
 //
 // Statistics, s before its rounding and all sums are fp32. As in add_rms_norm, the
-// forward normalises the unrounded s and the backward starts from the stored one.
+// forward normalises the unrounded s and the backward starts from the stored one (whose
+// rounding makes bf16 gradients 0.0024 off in the norm, where 0.0017 is their own).
+//
+// Measured, bf16: 32768 x 2048 with a gate a channel 101 us (5.3 TB/s, a copy's rate), its
+// gradient 168 us (4.8 TB/s) and 8 for the column sums; one row 3.5 us.
 #include <algorithm>
 
 #include "gemm.hpp"

@@ -17,6 +17,9 @@
 //     that lies inside is written, one that crosses an end leaves its part in the
 //     workspace (fp32). Further workgroups write the rows that no token names.
 //  3. The parts of the runs that cross, in order.
+//
+// Measured, bf16, 16384 tokens as text has them, 50000 ids of 2048 values: lookup 26 us
+// (5.1 TB/s), sort 18, sums and zeros 66 (4.1 TB/s), join 10.
 #include <algorithm>
 
 #include "gemm.hpp"

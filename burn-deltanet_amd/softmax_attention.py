@@ -56,7 +56,9 @@ def _ints(t: Tensor, n: int, what: str) -> Tensor:
         raise DeltaError(-7, f"{what}: expected int32 or int64, got {t.dtype}")
     if tuple(t.shape) != (n,):
         raise DeltaError(-2, f"{what}: expected [{n}], got {list(t.shape)}")
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check(q, k, v, offsets):

@@ -56,17 +56,11 @@ def _block_norm(x, residual, pre_weight, post_weight, gate, residual_scale, eps)
     pre = _vector(pre_weight, dim, None, "pre_weight")
     post = _vector(post_weight, dim, pre.dtype, "post_weight")
     kind, g = _gate(gate, x, rows, dim, pre.dtype, "gate")
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = abi.BlockNormArgs()
-    a.rows, a.dim, a.eps, a.residual_scale = rows, dim, float(eps), float(residual_scale)
-    a.dtype, a.weight_dtype, a.gate_kind = tag, abi.dtype_tag(pre.dtype), kind
-    a.x, a.x_stride = x2.data_ptr(), x2.stride(0)
-    a.residual, a.residual_stride = r2.data_ptr(), r2.stride(0)
-    a.pre_weight, a.post_weight = pre.data_ptr(), _p(post)
-    if g is not None:
-        a.gate, a.gate_stride = g.data_ptr(), g.stride(0)
-    a.sum, a.sum_stride, a.out, a.out_stride = total.data_ptr(), dim, out.data_ptr(), dim
+    out, total = x.new_empty(x.shape), x.new_empty(x.shape)
+    a = abi.BlockNormArgs(
+        rows, dim, x2.stride(0), r2.stride(0), 0 if g is None else g.stride(0), dim, dim, eps,
+        residual_scale, tag, abi.dtype_tag(pre.dtype), kind, x2.data_ptr(), r2.data_ptr(),
+        pre.data_ptr(), _p(post), _p(g), total.data_ptr(), out.data_ptr())
     _call("dn_block_norm", a, False, x.device)
     return out, total
 
@@ -170,12 +164,10 @@ def _embedding(tokens, table, scale):
     ids, (vocab, dim) = _ids(tokens), table.shape
     tag = abi.dtype_tag(table.dtype)
     t = _rows(table, "table")
-    out = torch.empty(tokens.shape + (dim,), dtype=table.dtype, device=table.device)
-    a = abi.EmbeddingArgs()
-    a.tokens, a.vocab, a.dim, a.scale = ids.numel(), vocab, dim, float(scale)
-    a.dtype, a.wide_ids = tag, int(ids.dtype == torch.int64)
-    a.ids, a.table, a.table_stride = ids.data_ptr(), t.data_ptr(), t.stride(0)
-    a.out, a.out_stride = out.data_ptr(), dim
+    out = table.new_empty(tokens.shape + (dim,))
+    a = abi.EmbeddingArgs(ids.numel(), vocab, dim, t.stride(0), dim, scale, tag,
+                          int(ids.dtype == torch.int64), ids.data_ptr(), t.data_ptr(),
+                          out.data_ptr())
     _call("dn_embedding", a, False, table.device)
     return out
 

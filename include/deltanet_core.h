@@ -594,7 +594,7 @@ int dn_block_norm_bwd(const dn_block_norm_bwd_args *args, hipStream_t stream);
 size_t dn_block_norm_bwd_workspace_bytes(const dn_block_norm_bwd_args *args);
 
 /* out[i] = scale * table[ids[i]]; an id outside [0, vocab) stands for a row of
- * zeros. Up to 2^28 tokens, a vocab up to 2^24. */
+ * zeros. Up to 2^28 tokens, a vocab up to 2^24, dim up to 2^23. */
 typedef struct {
   int64_t tokens, vocab, dim;
   int64_t table_stride, out_stride;
@@ -636,7 +636,8 @@ size_t dn_embedding_bwd_workspace_bytes(const dn_embedding_bwd_args *args);
  * that sees no key, and every row behind the last sequence, gets zeros, and -inf as its
  * log-sum. Keys that a row does not see have no influence on it, whatever they hold;
  * offsets and spans that leave the tensors are cut off at their ends. Scores, sums and
- * statistics are fp32. head_dim up to 256; (tokens + sequences) * nheads below 2^31. */
+ * statistics are fp32. head_dim up to 256; tokens * nheads / 64 + (sequences + 1) *
+ * kv_heads below 2^22. */
 typedef struct {
   int64_t tokens, key_rows, sequences, nheads, kv_heads, head_dim;
   int64_t q_stride, k_stride, v_stride, out_stride;

@@ -68,6 +68,8 @@ INF = float("inf")
     (EMB, dict(tokens=(1 << 28) + 1), -2, "tensor too large"),
     (EMB, dict(vocab=0), -2, "width"),
     (EMB, dict(vocab=(1 << 24) + 1), -2, "tensor too large"),
+    (EMB, dict(dim=(1 << 23) + 1, table_stride=1 << 24, out_stride=1 << 24), -2,
+     "tensor too large"),
     (EMB, dict(scale=INF), -2, "scale"),
     (EMB, dict(ids=None), -6, "ids is NULL"),
     (EMB, dict(table_stride=4), -2, "table"),
@@ -81,6 +83,7 @@ INF = float("inf")
     (ATT, dict(head_dim=0), -2, "head_dim"),
     (ATT, dict(head_dim=257), -9, "head_dim"),
     (ATT, dict(tokens=1 << 30), -2, "tensor too large"),
+    (ATT, dict(tokens=1 << 26, nheads=4, kv_heads=4), -2, "tensor too large"),
     (ATT, dict(sequences=1 << 29), -2, "tensor too large"),
     (ATT, dict(scale=0.0), -2, "scale"),
     (ATT, dict(scale=-1.0), -2, "scale"),
