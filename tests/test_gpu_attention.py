@@ -200,6 +200,35 @@ def test_spans_beyond_the_tensors():
         assert out.shape == q.shape
 
 
+def test_a_cache_past_32_bits():
+    """Rows whose first value is more than 2^32 bytes, and 2^31 values, from the start."""
+    rows, heads, kv, dim = 9_000_000, 4, 2, 128
+    gen = torch.Generator("cuda").manual_seed(13)
+    k = torch.empty(rows, kv, dim, dtype=BF, device="cuda")
+    v = torch.empty(rows, kv, dim, dtype=BF, device="cuda")
+    k[-700:], v[-700:] = made(gen, (700, kv, dim), BF), made(gen, (700, kv, dim), BF)
+    q = made(gen, (3, heads, dim), BF)
+    ints = lambda xs: torch.tensor(xs, dtype=torch.int32, device="cuda")
+    off, counts = ints([0, 1, 3]), ints([650, 300])
+    got = dn.attention(q, k, v, off, dn.KeySpans(ints([rows - 700, rows - 300]), counts))
+    want = dn.attention(q, k[-700:].clone(), v[-700:].clone(), off,
+                        dn.KeySpans(ints([0, 400]), counts))
+    # The split of the keys goes by the cache's size: the same sums in another order.
+    ref = su.attention(*wide(q, k[-700:], v[-700:]), [(0, 1, 0, 650), (1, 2, 400, 300)], None,
+                       True, BF)
+    check(got, ref["out"], "out")
+    check(want, ref["out"], "out of the short cache")
+
+
+def test_no_requests():
+    """A batch without requests over a cache."""
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    k = torch.ones(50, 2, 64, dtype=BF, device="cuda")
+    out = dn.attention(torch.empty(0, 1, 4, 64, dtype=BF, device="cuda"), k, k, None,
+                       dn.KeySpans(none, none))
+    assert out.shape == (0, 1, 4, 64)
+
+
 def test_nothing_there():
     empty = torch.empty(0, 4, 64, dtype=BF, device="cuda")
     off = torch.zeros(3, dtype=torch.int32, device="cuda")
