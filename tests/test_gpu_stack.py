@@ -199,7 +199,8 @@ def looked_up(tokens, vocab, dim, dtype, wide_ids, skew, seed=5):
     (100, 1009, 200, F32, True, "log"), (700, 3, 33, BF, False, "even"),
     (1024, 600, 1039, BF, True, "log"), (1025, 131073, 16, F32, True, "even"),
     (5000, 50000, 128, BF, True, "log"), (3001, 1009, 2056, F32, False, "log"),
-    (2048, 7, 4100, BF, True, "log"), (4097, 20, 72, F32, True, "one")])
+    (2048, 7, 4100, BF, True, "log"), (4097, 20, 72, F32, True, "one"),
+    (17001, 300, 2048, BF, True, "log"), (70000, 1000, 520, F32, True, "log")])
 def test_embedding(tokens, vocab, dim, dtype, wide_ids, skew):
     ids, table, d = looked_up(tokens, vocab, dim, dtype, wide_ids, skew)
     scale = 1.0 if dim == 64 else 2.5
