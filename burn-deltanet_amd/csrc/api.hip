@@ -1246,8 +1246,10 @@ int check_heads(int64_t tokens, int64_t sequences, int64_t nheads, int64_t kv_he
   if ((tokens * (nheads / kv_heads) / 64 + sequences + 1) * kv_heads >= (int64_t(1) << 22))
     return fail(DN_ERR_SHAPE, "tensor too large");
   if (!valid_dtype(dtype)) return fail(DN_ERR_DTYPE, "dtype must be DN_F32 or DN_BF16");
-  if (!std::isnan(scale) && !(scale > 0.0 && float(scale) > 0.f && std::isfinite(float(scale))))
-    return fail(DN_ERR_SHAPE, "scale must be a positive number");
+  // The kernels take exponents in powers of two: of scale · log2(e).
+  if (!std::isnan(scale) &&
+      !(scale > 0.0 && float(scale) > 0.f && std::isfinite(float(scale) * 1.442695041f)))
+    return fail(DN_ERR_SHAPE, "scale must be a positive number, finite times log2(e)");
   if (!offsets && tokens > 0 && (sequences < 1 || tokens % sequences))
     return fail(DN_ERR_SHAPE, "without offsets the sequences must have equal lengths");
   return DN_OK;
@@ -1271,11 +1273,17 @@ int check_attention(const dn_attention_args* a) {
   return check_rows(a->out, a->tokens, qd, a->out_stride, "out");
 }
 
+// Below, the log-sum over the scale, where the gradients' scores start, leaves fp32: the
+// log of the number of keys is below 21, which is 2^101 at this scale.
+constexpr double kLeastGradientScale = 0x1p-96;
+
 int check_attention_bwd(const dn_attention_bwd_args* a) {
   if (!a) return fail(DN_ERR_NULL, "args is NULL");
   if (int rc = check_heads(a->tokens, a->sequences, a->nheads, a->kv_heads, a->head_dim, a->dtype,
                            a->scale, a->offsets))
     return rc;
+  if (a->scale < kLeastGradientScale)
+    return fail(DN_ERR_UNSUPPORTED, "attention's gradients need a scale of at least 2^-96");
   const int64_t qd = a->nheads * a->head_dim, kd = a->kv_heads * a->head_dim;
   if (int rc = check_rows(a->q, a->tokens, qd, a->q_stride, "q")) return rc;
   if (int rc = check_rows(a->k, a->tokens, kd, a->k_stride, "k")) return rc;

@@ -21,6 +21,9 @@ from .autograd import first_order
 from .layer import _call, _gpu, _grows, _p
 
 
+LEAST_GRADIENT_SCALE = 2.0 ** -96  # dn_attention_bwd's (deltanet_core.h)
+
+
 class KeySpans(NamedTuple):
     """The rows of k and v that each sequence's queries attend to: lengths[s] rows from
     starts[s] on (int32, [sequences]). Spans may overlap, as where sequences share
@@ -136,13 +139,16 @@ def attention(q: Tensor, k: Tensor, v: Tensor, offsets: Optional[Tensor] = None,
     without it the operands are [batch, sequence, heads, dim]. Without `keys` a
     sequence's keys are its own rows; with it the queries are the last tokens over
     longer spans of a cache (no gradient). Causal: the i-th of n queries over m keys
-    sees keys 0 … i + m − n. scale: 1/sqrt(dim) unless given. A row that sees no key,
-    and every row behind the last sequence, is zeros; keys that a row does not see
-    have no influence on it, whatever they hold. The numbers in offsets and spans stay
-    on the GPU and are not checked: beyond the tensors' ends they are cut off."""
+    sees keys 0 … i + m − n. scale: 1/sqrt(dim) unless given; gradients need 2⁻⁹⁶ or
+    more. A row that sees no key, and every row behind the last sequence, is zeros;
+    keys that a row does not see have no influence on it, whatever they hold. The
+    numbers in offsets and spans stay on the GPU and are not checked: beyond the
+    tensors' ends they are cut off."""
     if _grows(q, k, v):
         if keys is not None:
             raise DeltaError(-9, "attention over key spans has no gradient")
+        if scale is not None and 0 < scale < LEAST_GRADIENT_SCALE:
+            raise DeltaError(-9, "attention's gradients need a scale of at least 2^-96")
         return _Attention.apply(q, k, v, offsets, scale, causal)
     return _attention(q, k, v, offsets, keys, scale, causal, False)[0]
 

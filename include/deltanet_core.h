@@ -641,7 +641,7 @@ size_t dn_embedding_bwd_workspace_bytes(const dn_embedding_bwd_args *args);
 typedef struct {
   int64_t tokens, key_rows, sequences, nheads, kv_heads, head_dim;
   int64_t q_stride, k_stride, v_stride, out_stride;
-  double scale;   /* above 0; NaN: 1/sqrt(head_dim) */
+  double scale;   /* above 0, scale * log2(e) finite in fp32; NaN: 1/sqrt(head_dim) */
   int32_t dtype;  /* q, k, v, out: DN_F32 or DN_BF16 */
   int32_t causal;
   const void *q, *k, *v;
@@ -663,7 +663,7 @@ typedef struct {
   int64_t tokens, sequences, nheads, kv_heads, head_dim;
   int64_t q_stride, k_stride, v_stride, out_stride, d_out_stride;
   int64_t d_q_stride, d_k_stride, d_v_stride;
-  double scale;
+  double scale;   /* as the forward's, and at least 2^-96 */
   int32_t dtype, causal;
   const void *q, *k, *v;
   const int32_t *offsets;

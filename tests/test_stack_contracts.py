@@ -1,0 +1,79 @@
+"""What attention, block_norm and embedding promise at the edges of what they accept:
+refusals, values that are not finite, sizes where a kernel's other form takes over."""
+
+import ctypes
+
+import pytest
+import torch
+
+import stack_util as su
+from conftest import load_package
+from layer_util import F, U, check
+from test_abi import fake_pointers
+from test_gpu_attention import check_all, made, packed, wide
+from test_stack_checks import ATT, ATT_BWD, FAKE
+
+dn = load_package()
+abi = dn.abi
+gpu = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def filled(entry, **over):
+    struct, _, sizes, pointers = entry
+    a = struct()
+    for k, v in {**sizes, **dict.fromkeys(pointers, FAKE), **over}.items():
+        setattr(a, k, v)
+    return a
+
+
+def refusal(entry, **over):
+    """The entry's code and message; nothing touches the device."""
+    L = abi.lib()
+    rc = getattr(L, entry[1])(ctypes.byref(filled(entry, **over)), None)
+    return rc, L.dn_last_error().decode()
+
+
+def ints(*xs):
+    return torch.tensor(xs, dtype=torch.int32, device="cuda")
+
+
+# -- attention: the scale ------------------------------------------------------------
+
+
+@fake_pointers
+def test_scales_that_leave_fp32_are_refused():
+    """Gradients start their scores at the log-sum over the scale, and all exponents are
+    taken of scale log2(e): both have to be fp32 numbers."""
+    for scale in (2.0 ** -97, 2e-38, 1e-40):
+        rc, message = refusal(ATT_BWD, scale=scale)
+        assert rc == -9 and "2^-96" in message
+        assert abi.lib().dn_attention_bwd_workspace_bytes(
+            ctypes.byref(filled(ATT_BWD, scale=scale))) == 0
+    for entry in (ATT, ATT_BWD):
+        rc, message = refusal(entry, scale=2.5e38)
+        assert rc == -2 and "scale" in message
+    # Within the limits the next check is reached.
+    small = dict(workspace=FAKE, workspace_bytes=8)
+    for scale in (2.0 ** -96, 2.3e38):
+        assert refusal(ATT_BWD, scale=scale, **small)[0] == -8
+
+
+@gpu
+def test_gradients_of_a_small_scale_are_refused_in_time():
+    """Before the forward, not in the backward pass."""
+    q = torch.ones(4, 1, 8, device="cuda", requires_grad=True)
+    with pytest.raises(dn.DeltaError, match="2\\^-96") as e:
+        dn.attention(q, q, q, ints(0, 4), None, 2.0 ** -97)
+    assert e.value.code == -9
+    assert dn.attention(q.detach(), q.detach(), q.detach(), ints(0, 4), None, 2.0 ** -97).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradients_at_the_smallest_scale(dtype):
+    """All weights are alike: d_v is a mean of d_out. Sums that start at the log-sum (6.9)
+    and take 64 products are off by 2 (64 + 4) u 6.9 = 940 u, for which the bound's term
+    for the weights' own sum, 2 (1000 + 8) u, has room."""
+    check_all(*packed([1000], 0, 1, 1, 64, dtype), scale=2.0 ** -96, causal=False)
