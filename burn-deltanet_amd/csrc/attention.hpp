@@ -233,10 +233,12 @@ struct Feed {
   static_assert(ROWS * TL::kWords % kNT == 0 && ROWS % kLong == 0, "whole words a thread");
   Rows<T> src;
   bool words, even;
+  bool repeat;  // what stands for rows that are not there: the last one, or zeros
   int64_t far;  // bytes of kLong rows
   uint32_t off[kD];
   bool on[kD];
-  __device__ inline Feed(const Rows<T>& rows, bool can_copy) : src(rows), words(can_copy) {
+  __device__ inline Feed(const Rows<T>& rows, bool can_copy, bool repeat_last = false)
+      : src(rows), words(can_copy), repeat(repeat_last) {
     const int g = src.group.size;
     even = 16 % g == 0;
     far = src.ld * int64_t(sizeof(T)) * (kLong / (even ? g : 1));
@@ -257,8 +259,7 @@ struct Feed {
       if (((e % TL::kWords) ^ M::template spread<HD>(e / TL::kWords)) * M::kCh >= src.dim)
         tile[e] = make_uint4(0, 0, 0, 0);
   }
-  // Rows from `first` (a multiple of ROWS) on, `there` (at least 1) of them; the others
-  // become zeros.
+  // Rows from `first` (a multiple of ROWS) on, `there` (at least 1) of them.
   __device__ inline void load(uint4* tile, int first, int there) const {
     if (words && even && there >= ROWS) {
       const char* base = scalar(reinterpret_cast<const char*>(src.base) +
@@ -282,7 +283,7 @@ struct Feed {
       const int e = i * kNT + int(threadIdx.x), r = e / TL::kWords;
       const int col = ((e % TL::kWords) ^ M::template spread<HD>(r)) * M::kCh;
       const T* row = src.at(first + min(r, there - 1));
-      if (r >= there || col >= src.dim) tile[e] = make_uint4(0, 0, 0, 0);
+      if ((r >= there && !repeat) || col >= src.dim) tile[e] = make_uint4(0, 0, 0, 0);
       else if (words) gemm::copy_to_lds(reinterpret_cast<const char*>(row + col), to + i * kNT * 16);
       else tile[e] = row_word(row, col, src.dim);
     }

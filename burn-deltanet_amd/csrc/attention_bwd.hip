@@ -272,10 +272,13 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
   const int first = p.causal ? jc * G : 0;
   const int whole = p.causal ? min(seq.len, j0 + S::kBM) * G - G : 0;
   const int b0 = p.causal ? j0 * G / BN : 0, count = (rows + BN - 1) / BN;
+  // Rows that are not there start their scores at −inf. Zeros as their queries would make
+  // that NaN for a key that is not finite; the last row's do so where that row, which sees
+  // every key, has NaN of its own.
   const Feed<T, HD, BN> queries(
       Rows<T>{static_cast<const T*>(p.q) + int64_t(seq.q0) * p.ldq + int64_t(head) * G * p.dim,
               p.ldq, p.dim, p.group},
-      p.words);
+      p.words, true);
   const Feed<T, HD, BN> cotangents(
       Rows<T>{static_cast<const T*>(p.d_out) + int64_t(seq.q0) * p.lddo +
                   int64_t(head) * G * p.dim,

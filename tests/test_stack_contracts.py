@@ -77,3 +77,34 @@ def test_gradients_at_the_smallest_scale(dtype):
     and take 64 products are off by 2 (64 + 4) u 6.9 = 940 u, for which the bound's term
     for the weights' own sum, 2 (1000 + 8) u, has room."""
     check_all(*packed([1000], 0, 1, 1, 64, dtype), scale=2.0 ** -96, causal=False)
+
+
+# -- attention: values that are not finite -------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 191])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [
+    (1, 1, 64, BF), (1, 1, 64, F32), (2, 1, 128, BF), (3, 1, 40, F32), (1, 1, 256, F32),
+    (1, 1, 256, BF), (2, 2, 128, F32)])
+def test_a_key_without_weight(rows, heads, kv, dim, dtype):
+    """A key whose scores are all -inf has a weight of zero: its d_k and d_v are zeros,
+    however many rows a tile lacks, and the other keys' are those of a batch whose rows
+    skip it."""
+    q, k, v, off, spans, do = packed([rows], 0, heads, kv, dim, dtype, seed=3)
+    q[:, :, 5] = (q[:, :, 5].abs() + 0.125).to(dtype)
+    at = 20
+    k[at, 0, 5] = -INF
+    for causal in (True, False):
+        out, lse = dn.attention_forward(q, k, v, off, None, None, causal)
+        assert out.isfinite().all() and lse.isfinite().all()
+        g = dn.attention_backward(do, q, k, v, out, lse, off, None, causal)
+        assert not g.d_k[at, 0].any() and not g.d_v[at, 0].any()
+        assert g.d_k.isfinite().all() and g.d_v.isfinite().all()
+        far = k.clone()  # a finite key as far away: the same weights of zero
+        far[at, 0] = 0
+        far[at, 0, 5] = -2e4
+        out2, lse2 = dn.attention_forward(q, far, v, off, None, None, causal)
+        want = dn.attention_backward(do, q, far, v, out2, lse2, off, None, causal)
+        assert torch.equal(out, out2) and torch.equal(lse, lse2)
+        assert torch.equal(g.d_k, want.d_k) and torch.equal(g.d_v, want.d_v)
