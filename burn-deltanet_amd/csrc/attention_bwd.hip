@@ -61,9 +61,11 @@ __global__ __launch_bounds__(kNT) void attention_stats_kernel(BwdArgs p) {
   }
 #pragma unroll
   for (int w = 8; w; w >>= 1) t += __shfl_xor(t, w);
+  // A row without a score above −inf was given zeros: its weights are zeros here too.
+  const float lse = p.lse[row];
   if (lane == 0)
     p.stats[(int64_t(kv) * p.spans.tokens + token) * p.group.size + (hd - kv * p.group.size)] =
-        make_float2(-p.lse[row] * kLog2E / p.c, -t);
+        make_float2(lse == -INFINITY ? lse : -lse * kLog2E / p.c, -t);
 }
 
 template <class T, int HD>

@@ -140,10 +140,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, offsets: Optional[Tensor] = None,
     sequence's keys are its own rows; with it the queries are the last tokens over
     longer spans of a cache (no gradient). Causal: the i-th of n queries over m keys
     sees keys 0 … i + m − n. scale: 1/sqrt(dim) unless given; gradients need 2⁻⁹⁶ or
-    more. A row that sees no key, and every row behind the last sequence, is zeros;
-    keys that a row does not see have no influence on it, whatever they hold. The
-    numbers in offsets and spans stay on the GPU and are not checked: beyond the
-    tensors' ends they are cut off."""
+    more. A row that sees no key, or none with a score above −inf, and every row behind
+    the last sequence, is zeros; keys that a row does not see have no influence on it,
+    whatever they hold. The numbers in offsets and spans stay on the GPU and are not
+    checked: beyond the tensors' ends they are cut off."""
     if _grows(q, k, v):
         if keys is not None:
             raise DeltaError(-9, "attention over key spans has no gradient")

@@ -633,9 +633,10 @@ size_t dn_embedding_bwd_workspace_bytes(const dn_embedding_bwd_args *args);
  * do not fall; NULL: `sequences` of tokens / sequences rows each. Its keys are the same
  * rows of k and v, or key_lengths[s] rows from key_starts[s] on (a cache; spans may
  * overlap). Causal: the i-th of n queries over m keys sees keys 0 ... i + m - n. A row
- * that sees no key, and every row behind the last sequence, gets zeros, and -inf as its
- * log-sum. Keys that a row does not see have no influence on it, whatever they hold;
- * offsets and spans that leave the tensors are cut off at their ends. Scores, sums and
+ * that sees no key, or none with a score above -inf, and every row behind the last
+ * sequence, gets zeros, and -inf as its log-sum; its weights are zeros in the gradients
+ * too. Keys that a row does not see have no influence on it, whatever they hold; offsets
+ * and spans that leave the tensors are cut off at their ends. Scores, sums and
  * statistics are fp32. head_dim up to 256; tokens * nheads / 64 + (sequences + 1) *
  * kv_heads below 2^22. */
 typedef struct {

@@ -108,3 +108,25 @@ def test_a_key_without_weight(rows, heads, kv, dim, dtype):
         want = dn.attention_backward(do, q, far, v, out2, lse2, off, None, causal)
         assert torch.equal(out, out2) and torch.equal(lse, lse2)
         assert torch.equal(g.d_k, want.d_k) and torch.equal(g.d_v, want.d_v)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_row_without_a_finite_score(dtype, dim):
+    """The first row sees the first key alone, with a score of -inf: zeros, a log-sum of
+    -inf, and no part in any gradient; the others are as if it were not there."""
+    q, k, v, off, spans, do = packed([70], 0, 1, 1, dim, dtype, seed=4)
+    q[:, :, 5] = (q[:, :, 5].abs() + 0.125).to(dtype)
+    k[0, 0, 5] = -INF
+    out, lse = dn.attention_forward(q, k, v, off)
+    assert not out[0].any() and lse[0] == -INF and lse[1:].isfinite().all()
+    g = dn.attention_backward(do, q, k, v, out, lse, off)
+    rest = [i for i in range(dim) if i != 5]  # 0 (-inf) there
+    assert not g.d_q[0, 0, rest].any() and not g.d_k[0].any() and not g.d_v[0].any()
+    one = [t[1:].clone() for t in (q, k, v)]
+    ref = su.attention(*wide(*one), [(0, 69, 0, 69)], None, True, dtype, do[1:].to(F))
+    check(out[1:], ref["out"], "out")
+    check(g.d_q[1:, 0][:, rest], tuple(t[:, 0][:, rest] for t in ref["d_q"]), "d_q")
+    check(g.d_k[1:], ref["d_k"], "d_k")
+    check(g.d_v[1:], ref["d_v"], "d_v")
