@@ -161,7 +161,9 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
       m = over_column<E>(m, [](float x, float y) { return fmaxf(x, y); }) * p.c;
       if (__any(m > top + kGrowth)) {
         const float now = fmaxf(top, m);
-        const float f = now == top ? 1.f : __builtin_amdgcn_exp2f(top - now);
+        // Not zero, which would make NaN of infinities that were set apart: 2^-126 of the
+        // sums so far is nothing beside a weight of one.
+        const float f = now == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(top - now), 0x1p-126f);
         top = now;
         sum *= f;
 #pragma unroll

@@ -130,3 +130,46 @@ def test_a_row_without_a_finite_score(dtype, dim):
     check(g.d_q[1:, 0][:, rest], tuple(t[:, 0][:, rest] for t in ref["d_q"]), "d_q")
     check(g.d_k[1:], ref["d_k"], "d_k")
     check(g.d_v[1:], ref["d_v"], "d_v")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [7, 64, 100, 300])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_an_infinite_value_that_a_row_sees(dtype, rows, dim):
+    """Weights are above zero: the sum is that infinity, in the tile where a row's keys
+    start as in later ones, and as the gradient of v the same; both infinities make NaN."""
+    q, k, v, off, spans, do = packed([rows], 0, 2, 1, dim, dtype, seed=5)
+    v[3, 0, 7], v[5, 0, 6], v[2, 0, 9], v[rows // 2 + 2, 0, 9] = INF, -INF, INF, -INF
+    for causal in (True, False):
+        out, lse = dn.attention_forward(q, k, v, off, None, None, causal)
+        first = lambda at: at if causal else 0
+        assert (out[first(3):, :, 7] == INF).all() and (out[first(5):, :, 6] == -INF).all()
+        both = first(rows // 2 + 2)
+        assert out[both:, :, 9].isnan().all() and (out[first(2):both, :, 9] == INF).all()
+        for at, col in ((3, 7), (5, 6), (2, 9)):
+            assert out[:first(at), :, col].isfinite().all()
+        rest = [i for i in range(dim) if i not in (6, 7, 9)]
+        tame = v.clone()
+        tame[:, 0, [6, 7, 9]] = 0
+        want, _ = dn.attention_forward(q, k, tame, off, None, None, causal)
+        assert torch.equal(out[..., rest], want[..., rest])
+    q, k, v, off, spans, do = packed([rows], 0, 2, 1, dim, dtype, seed=5)
+    out, lse = dn.attention_forward(q, k, v, off)
+    last = rows - 2
+    do[last, 1, 4] = -INF
+    g = dn.attention_backward(do, q, k, v, out, lse, off)
+    assert (g.d_v[:last + 1, 0, 4] == -INF).all() and g.d_v[last + 1, 0, 4].isfinite()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_an_infinite_value_at_the_largest_score(dtype):
+    """The key outweighs all before it by more than fp32 holds."""
+    q, k, v, off, spans, do = packed([70], 0, 1, 1, 64, dtype, seed=5)
+    q[:, 0, 0] = 8
+    k[:, 0, 0] = 0
+    k[66, 0, 0], v[66, 0, 3] = 400, INF  # a score of 400: 2^577 times the others' weights
+    out = dn.attention(q, k, v, off)
+    assert (out[66:, 0, 3] == INF).all() and out[:66].isfinite().all()
+    assert out[66:, 0, [i for i in range(64) if i != 3]].isfinite().all()
