@@ -129,7 +129,8 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_kernel(FwdAr
     const char* const tv = reinterpret_cast<const char*>(value_tile);
     if constexpr (kPartly) {
       if (__syncthreads_or(Feed<T, HD, BN>::wild(value_tile)))
-        set_apart<T, HD, BN, kNT, DB>(value_tile, o, h, [&](int j) { return n * BN + j <= last; });
+        set_apart<T, HD, BN, kNT, DB>(value_tile, o, h, 1.f,
+                                      [&](int j) { return n * BN + j <= last; });
     }
     // At 256 values a head some operands come back from scratch memory, which waits for
     // every copy issued before: the copies go behind the scores.

@@ -357,9 +357,11 @@ __device__ inline float over_column(float v, F f) {
 // them, as 0 · inf. Their rows' part of the columns that do see them (which are then
 // not finite in any case) is added here, value by value, and the tile loses them.
 // For whole workgroups; the tile may be used when it returns. `sees(row)`: whether
-// the lane's column does.
+// the lane's column does. `weight` stands for theirs: 1 for a softmax's, which are above
+// zero; 0 for dS of a key or query that is not finite, which is 0 or NaN.
 template <class T, int HD, int ROWS, int NT, int NB, class Sees>
-__device__ void set_apart(uint4* tile, typename Mma<T>::Acc (&acc)[NB], int h, Sees sees) {
+__device__ void set_apart(uint4* tile, typename Mma<T>::Acc (&acc)[NB], int h, float weight,
+                          Sees sees) {
   using M = Mma<T>;
   for (int r = 0; r < ROWS; ++r) {
     const bool on = sees(r);
@@ -368,7 +370,7 @@ __device__ void set_apart(uint4* tile, typename Mma<T>::Acc (&acc)[NB], int h, S
 #pragma unroll
       for (int i = 0; i < M::kAcc; ++i) {
         const float v = Tile<T, HD>::value(tile, r, b * M::kE + M::row(i, h));
-        if (on && !(fabsf(v) < INFINITY)) acc[b][i] += v;
+        if (on && !(fabsf(v) < INFINITY)) acc[b][i] += v * weight;
       }
   }
   __syncthreads();

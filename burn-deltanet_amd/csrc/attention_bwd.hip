@@ -233,7 +233,8 @@ __global__ __launch_bounds__(kNT, HD <= 128 ? 2 : 1) void attention_dq_kernel(Bw
     if (S::kLarge && n + 1 < count) load(n + 1, buf ^ 1);
     if constexpr (kPartly) {
       if (__syncthreads_or(Feed<T, HD, BN>::wild(key_tile)))
-        set_apart<T, HD, BN, kNT, DB>(key_tile, dq, h, [&](int j) { return n * BN + j <= last; });
+        set_apart<T, HD, BN, kNT, DB>(key_tile, dq, h, 0.f,
+                                      [&](int j) { return n * BN + j <= last; });
     }
     if (active) {
       gradient(B0{}, [&](auto i) {
@@ -427,8 +428,9 @@ __device__ inline void key_gradients(const BwdArgs& p, uint4* smem, float* stats
                       (DV ? Feed<T, HD, BN>::wild(query_tile + S::kTileWords) : 0);
       if (__syncthreads_or(bad)) {
         const auto sees = [&](int i) { return n * BN + i >= first; };
-        if constexpr (DK) set_apart<T, HD, BN, kNT, DB>(query_tile, dk, h, sees);
-        if constexpr (DV) set_apart<T, HD, BN, kNT, DB>(query_tile + S::kTileWords, dv, h, sees);
+        if constexpr (DK) set_apart<T, HD, BN, kNT, DB>(query_tile, dk, h, 0.f, sees);
+        if constexpr (DV)
+          set_apart<T, HD, BN, kNT, DB>(query_tile + S::kTileWords, dv, h, 1.f, sees);
       }
     }
     if (active) {

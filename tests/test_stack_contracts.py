@@ -173,3 +173,17 @@ def test_an_infinite_value_at_the_largest_score(dtype):
     out = dn.attention(q, k, v, off)
     assert (out[66:, 0, 3] == INF).all() and out[:66].isfinite().all()
     assert out[66:, 0, [i for i in range(64) if i != 3]].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_query_that_sees_an_infinite_key(dtype, dim):
+    """dS is 0 there, and 0 inf is NaN, in tiles that a row sees whole as in the others."""
+    q, k, v, off, spans, do = packed([200], 0, 2, 1, dim, dtype, seed=6)
+    q[:, :, 5] = (q[:, :, 5].abs() + 0.125).to(dtype)
+    k[20, 0, 5] = -INF
+    out, lse = dn.attention_forward(q, k, v, off)
+    g = dn.attention_backward(do, q, k, v, out, lse, off)
+    assert g.d_q[20:, :, 5].isnan().all() and g.d_q[:20].isfinite().all()
+    assert g.d_q[..., [i for i in range(dim) if i != 5]].isfinite().all()
