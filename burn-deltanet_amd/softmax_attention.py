@@ -64,8 +64,9 @@ def _ints(t: Tensor, n: int, what: str) -> Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _check(q, k, v, offsets):
-    """The operands as rows, and how many sequences they hold."""
+def _check(q, k, v, offsets, spans):
+    """The operands as rows, and how many sequences they hold. `spans`: whether the keys
+    are others than the queries' rows."""
     for t, what in ((k, "k"), (v, "v")):
         if t.dtype != q.dtype:
             raise DeltaError(-7, f"{what}: expected {q.dtype}, got {t.dtype}")
@@ -74,6 +75,10 @@ def _check(q, k, v, offsets):
     if k3.shape != v3.shape or k3.shape[2] != q3.shape[2]:
         raise DeltaError(-2, f"k, v: expected [..., heads, {q3.shape[2]}] of one shape, "
                              f"got {list(k.shape)} and {list(v.shape)}")
+    if not spans and (k3.shape[0] != q3.shape[0]
+                      or (offsets is None and k.shape[:-2] != q.shape[:-2])):
+        raise DeltaError(-2, f"k, v: expected the queries' rows {list(q.shape[:-2])} without key "
+                             f"spans, got {list(k.shape[:-2])}")
     if offsets is None:
         if q.dim() != 4:
             raise DeltaError(-2, "q: expected [batch, sequence, heads, dim] without offsets")
@@ -85,15 +90,12 @@ def _check(q, k, v, offsets):
 
 
 def _attention(q, k, v, offsets, keys, scale, causal, keep):
-    q3, k3, v3, off, n = _check(q, k, v, offsets)
+    q3, k3, v3, off, n = _check(q, k, v, offsets, keys is not None)
     a = abi.AttentionArgs()
     if keys is not None:
         starts = _ints(keys.starts, n, "keys.starts")
         lengths = _ints(keys.lengths, n, "keys.lengths")
         a.key_starts, a.key_lengths = starts.data_ptr(), lengths.data_ptr()
-    elif k3.shape[0] != q3.shape[0] or (offsets is None and k.shape[:-2] != q.shape[:-2]):
-        raise DeltaError(-2, f"k, v: expected the queries' rows {list(q.shape[:-2])} without key "
-                             f"spans, got {list(k.shape[:-2])}")
     a.tokens, a.nheads, a.head_dim = q3.shape
     a.key_rows, a.kv_heads, a.sequences = k3.shape[0], k3.shape[1], n
     a.scale, a.causal, a.dtype = nan_scale(scale), int(bool(causal)), abi.dtype_tag(q.dtype)
@@ -166,10 +168,7 @@ def attention_backward(d_out: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tens
                        causal: bool = True, need_q: bool = True, need_k: bool = True,
                        need_v: bool = True) -> AttentionGrads:
     """The gradients of attention without key spans."""
-    q3, k3, v3, off, n = _check(q, k, v, offsets)
-    if k3.shape[0] != q3.shape[0]:
-        raise DeltaError(-2, f"k, v: expected the queries' rows {list(q.shape[:-2])}, "
-                             f"got {list(k.shape[:-2])}")
+    q3, k3, v3, off, n = _check(q, k, v, offsets, False)
     for t, what in ((d_out, "d_out"), (out, "out")):
         if t.dtype != q.dtype:
             raise DeltaError(-7, f"{what}: expected {q.dtype}, got {t.dtype}")

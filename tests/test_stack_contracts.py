@@ -187,3 +187,22 @@ def test_a_query_that_sees_an_infinite_key(dtype, dim):
     g = dn.attention_backward(do, q, k, v, out, lse, off)
     assert g.d_q[20:, :, 5].isnan().all() and g.d_q[:20].isfinite().all()
     assert g.d_q[..., [i for i in range(dim) if i != 5]].isfinite().all()
+
+
+# -- attention: shapes ---------------------------------------------------------------
+
+
+@gpu
+def test_both_halves_refuse_keys_of_another_batch():
+    """As many rows as q, but in other sequences."""
+    on = lambda *shape: torch.ones(shape, device="cuda")
+    q, k = on(2, 6, 2, 8), on(3, 4, 2, 8)
+    for call in (lambda: dn.attention(q, k, k), lambda: dn.attention_forward(q, k, k),
+                 lambda: dn.attention_backward(q, q, k, k, q, on(2, 6, 2))):
+        with pytest.raises(dn.DeltaError, match="without key spans") as e:
+            call()
+        assert e.value.code == -2
+    # With offsets only the rows count, as in the forward.
+    off = ints(0, 6, 12)
+    out, lse = dn.attention_forward(q, k, k, off)
+    assert dn.attention_backward(q, q, k, k, out, lse, off).d_k.shape == k.shape
