@@ -1264,7 +1264,8 @@ int check_attention(const dn_attention_args* a) {
     return fail(DN_ERR_NULL, "key_starts and key_lengths go together");
   if (a->key_rows < 0 || a->key_rows > INT32_MAX / 2)
     return fail(DN_ERR_SHAPE, "key_rows out of range");
-  if (!a->key_starts && a->key_rows != a->tokens)
+  // Without sequences no key is read, and spans may have no address.
+  if (!a->key_starts && a->sequences > 0 && a->key_rows != a->tokens)
     return fail(DN_ERR_SHAPE, "without key spans k and v must have the queries' rows");
   const int64_t qd = a->nheads * a->head_dim, kd = a->kv_heads * a->head_dim;
   if (int rc = check_rows(a->q, a->tokens, qd, a->q_stride, "q")) return rc;

@@ -206,3 +206,25 @@ def test_both_halves_refuse_keys_of_another_batch():
     off = ints(0, 6, 12)
     out, lse = dn.attention_forward(q, k, k, off)
     assert dn.attention_backward(q, q, k, k, out, lse, off).d_k.shape == k.shape
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_padding_without_requests(dtype):
+    """Rows of padding over a cache, and no request: zeros, whatever the cache holds."""
+    gen = torch.Generator("cuda").manual_seed(7)
+    q, cache = made(gen, (9, 4, 64), dtype), made(gen, (50, 2, 64), dtype)
+    cache[:] = NAN
+    none = dn.KeySpans(ints(), ints())
+    out, lse = dn.attention_forward(q, cache, cache, ints(0), none)
+    assert out.shape == q.shape and not out.any() and (lse == -INF).all()
+    out = dn.attention(q[:0], cache, cache, ints(0), none)
+    assert out.shape == (0, 4, 64)
+    with pytest.raises(dn.DeltaError, match="multiple"):  # empty calls are checked too
+        dn.attention(q[:0, :3], cache, cache, ints(0), none)
+
+
+@fake_pointers
+def test_key_rows_without_sequences():
+    assert refusal(ATT, tokens=0, sequences=0, key_rows=9)[0] == 0
+    assert refusal(ATT, tokens=0, sequences=1, key_rows=9)[0] == -2
