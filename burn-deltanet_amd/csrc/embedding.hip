@@ -75,6 +75,12 @@ struct SortArgs {
   int tokens, vocab, width;  // width: ids of a workgroup
 };
 
+// Between accesses of a wave's lanes to each other's values in LDS.
+__device__ inline void lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <class ID>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs p) {
   extern __shared__ int counts[];  // [waves][width]
@@ -161,13 +167,18 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs p
         const uint64_t all = __ballot(set);
         same &= set ? all : ~all;
       }
+      const int rank = int(__popcll(same & ((uint64_t(1) << lane) - 1)));
+      int at = 0;
       if (in) {
-        const int rank = int(__popcll(same & ((uint64_t(1) << lane) - 1)));
-        const int at = mine[key] + rank;
+        at = mine[key] + rank;
         p.pos[at] = int(i0 + 64 * j + lane);
         p.key[at] = lo + key;
-        if (rank == 0) mine[key] = at + int(__popcll(same));
       }
+      // The first lane of an id moves its place on: behind the others' reads, and before
+      // those of the next step.
+      lds_fence();
+      if (in && rank == 0) mine[key] = at + int(__popcll(same));
+      lds_fence();
     }
   }
 }

@@ -228,3 +228,23 @@ def test_padding_without_requests(dtype):
 def test_key_rows_without_sequences():
     assert refusal(ATT, tokens=0, sequences=0, key_rows=9)[0] == 0
     assert refusal(ATT, tokens=0, sequences=1, key_rows=9)[0] == -2
+
+
+# -- embedding -----------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,wide_ids", [(64, 2, True), (5000, 3, False),
+                                                   (20000, 1, True), (33333, 700, True),
+                                                   (40000, 140000, False)])
+def test_every_token_counts_once(tokens, vocab, wide_ids):
+    """Whole numbers below 2^24 in the sums: fp32 holds them exactly, so that a token that
+    is lost or taken twice shows."""
+    gen = torch.Generator("cuda").manual_seed(8)
+    ids = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    ids[::3] = vocab - 1  # many lanes of a step share an id
+    d = torch.randint(-9, 10, (tokens, 24), generator=gen, device="cuda")
+    d[:, 0] = 1
+    want = torch.zeros(vocab, 24, dtype=torch.long, device="cuda").index_add(0, ids, d)
+    got = dn.embedding_backward(d.float(), ids if wide_ids else ids.int(), vocab)
+    assert torch.equal(got.long(), want) and torch.equal(got, got.round())
