@@ -248,3 +248,31 @@ def test_every_token_counts_once(tokens, vocab, wide_ids):
     want = torch.zeros(vocab, 24, dtype=torch.long, device="cuda").index_add(0, ids, d)
     got = dn.embedding_backward(d.float(), ids if wide_ids else ids.int(), vocab)
     assert torch.equal(got.long(), want) and torch.equal(got, got.round())
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [9, 16, 8 * 64, 8 * 65, 8 * 66 + 3, 8 * 129, 4096, 4097,
+                                    32 * 193 + 1, 32 * 4161])
+def test_ids_of_many_parts(tokens):
+    """One id between two others, of up to thousands of the sums that are joined: as many
+    as are looked for at a time, one more, one less, and at a second level."""
+    gen = torch.Generator("cuda").manual_seed(9)
+    d = torch.randint(-9, 10, (tokens, 5), generator=gen, device="cuda")
+    for before, behind in ((0, 0), (1, 1), (33, 40), (tokens // 2, 1), (tokens - 9, 0)):
+        ids = torch.ones(tokens, dtype=torch.long, device="cuda")
+        ids[:before] = 0
+        ids[tokens - behind:] = 2
+        want = torch.zeros(3, 5, dtype=torch.long, device="cuda").index_add(0, ids, d)
+        got = dn.embedding_backward(d.float(), ids, 3)
+        assert torch.equal(got.long(), want) and torch.equal(got, got.round())
+
+
+@gpu
+def test_many_tokens_of_few_values_leave_few_parts():
+    """Sums of 32 tokens, however little there is to do: a join of four times the parts
+    took up to 2.4 times as long."""
+    a = filled((abi.EmbeddingBwdArgs, "dn_embedding_bwd",
+                dict(tokens=65536, vocab=300, dim=64, d_out_stride=64, d_table_stride=64,
+                     scale=1.0), ["ids", "d_out", "d_table"]))
+    n = abi.lib().dn_embedding_bwd_workspace_bytes(ctypes.byref(a))
+    assert n <= 2 * 65536 * 4 + 65536 // 32 * 2 * 64 * 4 + 4096
