@@ -276,3 +276,205 @@ def test_many_tokens_of_few_values_leave_few_parts():
                      scale=1.0), ["ids", "d_out", "d_table"]))
     n = abi.lib().dn_embedding_bwd_workspace_bytes(ctypes.byref(a))
     assert n <= 2 * 65536 * 4 + 65536 // 32 * 2 * 64 * 4 + 4096
+
+
+# -- attention: forms that sizes choose ----------------------------------------------
+
+
+@gpu
+def test_gradients_at_large_scores(monkeypatch):
+    """Scores up to a few hundred. The gradients of the keys start their sums at the
+    log-sum over the scale: its magnitude is one more term of the product's, 2 (D + 4) u
+    of it beside the log-sum's own bound."""
+    head = su.head
+
+    def started(q, *rest):
+        f = head(q, *rest)
+        f["elses"] = f["elses"] + 2 * (q.shape[1] + 4) * U * f["lse"].abs()
+        return f
+
+    monkeypatch.setattr(su, "head", started)
+    for dtype in (BF, F32):
+        for dim in (64, 128, 256):
+            q, k, v, off, spans, do = packed([200, 140], 0, 2, 1, dim, dtype)
+            k = (k.float() * torch.linspace(0.1, 12, 340, device="cuda")[:, None, None]).to(dtype)
+            check_all(q, k, v, off, spans, do, scale=1.0)
+
+
+def cus():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def crowd(kv, per_tile, dtype, dim, group=2, seed=10):
+    """Enough short sequences for the gradients of keys and values to be formed together:
+    two workgroups a CU, of `per_tile` keys each."""
+    n = 2 * cus() // kv + 1
+    lengths = [(37 * i) % 90 + 1 for i in range(n - 2)] + [0, 3 * per_tile + 7]
+    t = packed(lengths, 5, group * kv, kv, dim, dtype, seed)
+    assert (t[0].shape[0] // per_tile + n + 1) * kv >= 2 * cus()
+    return t
+
+
+@gpu
+@pytest.mark.parametrize("kv,dim,dtype,group,causal", [
+    (16, 64, BF, 2, True), (16, 40, BF, 1, False), (16, 40, F32, 3, True),
+    (16, 128, F32, 1, True), (16, 128, F32, 2, False), (16, 33, BF, 1, True)])
+def test_d_k_and_d_v_together(kv, dim, dtype, group, causal):
+    q, k, v, off, spans, do = crowd(kv, 128 if dtype == BF else 64, dtype, dim, group)
+    check_all(q, k, v, off, spans, do, causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, BF), (128, F32)])
+@pytest.mark.parametrize("what", [NAN, INF])
+def test_later_keys_of_rows_that_are_not_finite(dim, dtype, what):
+    """d_k and d_v formed together: a row reaches no later key, and no other sequence."""
+    q, k, v, off, spans, do = crowd(16, 128 if dtype == BF else 64, dtype, dim)
+    out, lse = dn.attention_forward(q, k, v, off)
+    g = dn.attention_backward(do, q, k, v, out, lse, off)
+    first, n = spans[-1][:2]
+    at = first + n // 2
+    do[at, 1, 3], do[at, 5, 2] = what, what
+    q[at, 1, 4], q[at, 7, 2] = what, what
+    g2 = dn.attention_backward(do, q, k, v, out, lse, off)
+    same = torch.ones(q.shape[0], dtype=torch.bool, device="cuda")
+    same[first:at + 1] = False
+    for name in ("d_k", "d_v"):
+        a, b = getattr(g, name), getattr(g2, name)
+        assert torch.equal(a[same], b[same])
+        assert torch.equal(a[:, 4:], b[:, 4:])  # other key heads
+    assert not g2.d_v[first:at + 1, 0, 3].isfinite().any()
+    assert not g2.d_k[first:at + 1, 3].isfinite().all(-1).any()
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype,many", [(64, BF, True), (64, BF, False), (128, BF, False),
+                                            (40, F32, True), (128, F32, True), (256, F32, False),
+                                            (256, BF, False)])
+def test_one_gradient_at_a_time(dim, dtype, many):
+    q, k, v, off, spans, do = (crowd(16, 128 if dtype == BF else 64, dtype, dim, 1) if many
+                               else packed([150, 1, 0, 77], 3, 4, 2, dim, dtype))
+    out, lse = dn.attention_forward(q, k, v, off)
+    ref = su.attention(*wide(q, k, v), spans, None, True, dtype, do.to(F))
+    for names in (["d_q"], ["d_k"], ["d_v"], ["d_q", "d_v"], ["d_k", "d_v"]):
+        need = {f"need_{n}": f"d_{n}" in names for n in "qkv"}
+        g = dn.attention_backward(do, q, k, v, out, lse, off, **need)
+        for name in ("d_q", "d_k", "d_v"):
+            if name in names:
+                check(getattr(g, name), ref[name], name)
+            else:
+                assert getattr(g, name) is None
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,dtype", [(256, 1, BF), (60, 3, BF), (100, 1, F32)])
+def test_large_groups(heads, kv, dtype):
+    """More heads of a group than rows of a tile, and numbers that share no factor with it."""
+    check_all(*packed([70, 1, 3], 2, heads, kv, 64, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,dim,dtype,new", [
+    (4, 1, 128, BF, 3), (2, 2, 64, F32, 5), (6, 2, 40, BF, 1), (8, 1, 256, BF, 2),
+    (3, 1, 128, F32, 70), (4, 4, 33, BF, 2)])
+def test_split_keys(heads, kv, dim, dtype, new):
+    """Keys that are split among workgroups: several new tokens, spans of very different
+    lengths that end inside a tile, parts without a key, and values that are not finite
+    where no row looks and where all do."""
+    gen = torch.Generator("cuda").manual_seed(11)
+    rows = 6000
+    k, v = made(gen, (rows, kv, dim), dtype), made(gen, (rows, kv, dim), dtype)
+    spans = [(0, 4999), (4900, 300), (5500, new - 1)]
+    used = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for a, n in spans:
+        used[a:a + n] = True
+    k[~used], v[~used] = NAN, INF
+    n = len(spans)
+    assert 2 * cus() // (n * kv) >= 2 and rows // n // 256 >= 2  # more than one part
+    q = made(gen, (n * new, heads, dim), dtype)
+    keys = dn.KeySpans(ints(*(a for a, _ in spans)), ints(*(m for _, m in spans)))
+    offsets = ints(*(i * new for i in range(n + 1)))
+    where = [(i * new, new, a, m) for i, (a, m) in enumerate(spans)]
+    for causal in (True, False):
+        out, lse = dn.attention_forward(q, k, v, offsets, keys, None, causal)
+        ref = su.attention(*wide(q, k, v), where, None, causal, dtype)
+        check(out, ref["out"], "out")
+        seen = ref["lse"][0] > -INF
+        assert torch.equal(lse > -INF, seen)
+        check(lse[seen], (ref["lse"][0][seen], ref["lse"][1][seen]), "lse")
+        hot = v.clone()
+        hot[2500, 0, 5] = INF  # seen by the first request's rows alone
+        got = dn.attention(q, k, hot, offsets, keys, None, causal)
+        group = heads // kv
+        assert (got[:new, :group, 5] == INF).all()
+        got[:new, :group, 5] = out[:new, :group, 5]
+        assert torch.equal(got, out)
+
+
+# -- block_norm ----------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dim", [96, 1024, 4096, 9000])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_sum_over_an_input(dim, dtype, over):
+    """`sum` may lie on x or on the residual."""
+    gen = torch.Generator("cuda").manual_seed(12)
+    x, r = made(gen, (37, dim), dtype), made(gen, (37, dim), dtype)
+    pre, post, gate = (made(gen, (dim,), dtype) for _ in range(3))
+    want, total = dn.block_norm(x, r, pre, post, gate, 0.5)
+    out, to = torch.empty_like(x), x if over == "x" else r
+    a = abi.BlockNormArgs(37, dim, dim, dim, dim, dim, dim, 1e-5, 0.5, abi.dtype_tag(dtype),
+                          abi.dtype_tag(dtype), abi.DN_GATE_CHANNEL, x.data_ptr(), r.data_ptr(),
+                          pre.data_ptr(), post.data_ptr(), gate.data_ptr(), to.data_ptr(),
+                          out.data_ptr())
+    assert abi.lib().dn_block_norm(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(to, total) and torch.equal(out, want)
+
+
+# -- differentiation -----------------------------------------------------------------
+
+
+def operators():
+    gen = torch.Generator("cuda").manual_seed(13)
+    t = lambda *shape: made(gen, shape, F32)
+    off, tokens = ints(0, 7, 12), torch.arange(12, device="cuda") % 5
+    return {
+        "attention": (lambda q, k, v: dn.attention(q, k, v, off),
+                      (t(12, 4, 16), t(12, 2, 16), t(12, 2, 16))),
+        "block_norm": (lambda *a: dn.block_norm(*a)[0],
+                       (t(12, 24), t(12, 24), t(24), t(24), t(12, 1))),
+        "embedding": (lambda table: dn.embedding(tokens, table), (t(5, 24),))}
+
+
+@gpu
+@pytest.mark.parametrize("name", ["attention", "block_norm", "embedding"])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_tangents_are_refused(name, grad_mode):
+    fn, leaves = operators()[name]
+    ad = torch.autograd.forward_ad
+    with ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        want = fn(*leaves)  # no tangents: as ever
+        for i in range(len(leaves)):
+            dual = list(leaves)
+            dual[i] = ad.make_dual(leaves[i], torch.ones_like(leaves[i]))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                fn(*dual)
+    assert torch.equal(fn(*leaves), want)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["attention", "block_norm", "embedding"])
+def test_gradients_of_one_leaf_at_a_time(name):
+    """Other leaves' gradients are not asked for: the same numbers."""
+    fn, leaves = operators()[name]
+    every = [t.clone().requires_grad_(True) for t in leaves]
+    out = fn(*every)
+    c = torch.randn_like(out)
+    want = torch.autograd.grad(out, every, c)
+    for i, leaf in enumerate(leaves):
+        one = list(leaves)
+        one[i] = leaf.clone().requires_grad_(True)
+        got, = torch.autograd.grad(fn(*one), one[i], c)
+        assert torch.equal(got, want[i])
