@@ -35,10 +35,10 @@ class BlockNormGrads(NamedTuple):
 def _gate(gate: Optional[Tensor], x: Tensor, rows: int, dim: int, weight_dtype, what: str):
     """The gate's kind and the tensor that the kernel reads: [dim] in the weights'
     type, one value a row ([..., 1]) or x's shape in x's type. Where dim is 1 a
-    gate [..., 1] is x's shape."""
+    gate [..., 1] is x's shape; where x is [dim] one of the weights' type is a channel's."""
     if gate is None:
         return abi.DN_GATE_NONE, None
-    if gate.dim() == 1 and x.dim() != 1:
+    if gate.dim() == 1 and (x.dim() != 1 or (gate.shape[0] == dim and gate.dtype == weight_dtype)):
         return abi.DN_GATE_CHANNEL, _vector(gate, dim, weight_dtype, what)
     if gate.dim() and gate.shape[-1] == 1 and dim != 1 and gate.numel() == rows:
         return abi.DN_GATE_TOKEN, _like(gate, x, (rows, 1), what)

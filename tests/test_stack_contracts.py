@@ -433,6 +433,30 @@ def test_sum_over_an_input(dim, dtype, over):
     assert torch.equal(to, total) and torch.equal(out, want)
 
 
+@gpu
+@pytest.mark.parametrize("dtype,wdtype", [(BF, F32), (F32, BF), (F32, F32)])
+def test_gates_of_a_lone_row(dtype, wdtype):
+    """x [dim]: every kind of gate, as for x [1, dim]."""
+    gen = torch.Generator("cuda").manual_seed(14)
+    x, r, dy, full = (made(gen, (40,), dtype) for _ in range(4))
+    pre, channel = made(gen, (40,), wdtype), made(gen, (40,), wdtype)
+    token = made(gen, (1,), dtype)
+    for gate, shape in ((None, None), (channel, (40,)), (full, (1, 40)), (token, (1, 1))):
+        if gate is full and dtype == wdtype:
+            continue  # the same as a channel's
+        alone = gate if gate is None else gate.clone()
+        same = None if gate is None else gate.reshape(shape)
+        out, total = dn.block_norm(x, r, pre, None, alone)
+        want, ref = dn.block_norm(x[None], r[None], pre, None, same)
+        assert out.shape == (40,) and torch.equal(out, want[0]) and torch.equal(total, ref[0])
+        g = dn.block_norm_backward(dy, None, x, total, pre, None, alone)
+        h = dn.block_norm_backward(dy[None], None, x[None], ref, pre, None, same)
+        assert torch.equal(g.d_x, h.d_x[0]) and torch.equal(g.d_pre_weight, h.d_pre_weight)
+        if gate is not None:
+            assert g.d_gate.shape == gate.shape and g.d_gate.dtype == gate.dtype
+            assert torch.equal(g.d_gate, h.d_gate.reshape(gate.shape))
+
+
 # -- differentiation -----------------------------------------------------------------
 
 
