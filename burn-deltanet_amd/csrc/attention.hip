@@ -18,12 +18,13 @@
 // matrix unit (their sum is not), the output once.
 //
 // Bound by the matrix and the vector unit in turn, which two waves a SIMD overlap only in
-// part. Measured, bf16, 16 heads on 4 of 128: one causal sequence of 16384 1.13 ms (0.97
-// PFLOP/s); one token over 65536 keys 50 us and 13 for the join (2.7 TB/s), 64 over 2048
-// to 8192 each 182 us (3.8 TB/s: a CU has 64 KB of keys in flight). Through registers in
-// place of copies the first took 1.45 ms. Heads of other widths are padded in LDS to 64,
-// 128 or 256; widths that are no multiple of 16 bytes are read without copies, and the
-// tile's loads are not hidden (2048 tokens of 33 values: 119 us).
+// part. Measured, bf16, 16 heads on 4 of 128: one causal sequence of 16384 1.13 ms a call
+// (0.97 PFLOP/s; 1.24 under the tracer); one token over 65536 keys 50 us and 13 for the
+// join (2.7 TB/s), 64 over 2048 to 8192 each 182 us (3.8 TB/s: a CU has 64 KB of keys in
+// flight). Through registers in place of copies the first took 1.45 ms. Heads of other
+// widths are padded in LDS to 64, 128 or 256; widths that are no multiple of 16 bytes are
+// read without copies, and the tile's loads are not hidden (2048 tokens of 33 values: 119
+// us).
 #include <algorithm>
 
 #include "attention.hpp"

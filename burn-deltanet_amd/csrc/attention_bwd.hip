@@ -3,21 +3,22 @@
 // and dS = P ⊙ (dP − δ):
 //   d_q = scale·dS k,  d_k = scale·dSᵀ q,  d_v = Pᵀ d_out.
 //
-// Three launches: δ (with lse beside it, the rows of a group side by side); d_q, a workgroup a tile of rows that walks the keys; d_k and d_v, a workgroup
-// a tile of keys that walks the rows of all of its group's heads. So every gradient
-// is summed by one workgroup in a fixed order, without atomics, and a group's shared
-// heads need no sum of their own; the price is that S and dP are formed twice (seven
-// products in place of five). Every product leaves its sums where the next one takes
-// them as an operand (attention.hpp).
+// Three launches: δ (with lse beside it, the rows of a group side by side); d_q, a
+// workgroup a tile of rows that walks the keys; d_k and d_v, a workgroup a tile of keys
+// that walks the rows of all of its group's heads. So every gradient is summed by one
+// workgroup in a fixed order, without atomics, and a group's shared heads need no sum of
+// their own; the price is that S and dP are formed twice (seven products in place of
+// five), and S a third time (eight) where d_k and d_v are apart. Every product leaves its
+// sums where the next one takes them as an operand (attention.hpp).
 //
-// Sums are fp32; in bf16 the matrix unit takes P and dS rounded (the gradients are 0.0025
-// from a 64-bit result in the norm, where rounding the result alone gives 0.0017), the
-// gradients are rounded once.
+// Sums are fp32; in bf16 the matrix unit takes P and dS rounded, δ is that of the rounded
+// out, and the gradients are rounded once (they are 0.0025 from a 64-bit result in the
+// norm, up to 0.0035 where sequences are short, and rounding the result alone gives 0.0017).
 //
 // Bound by the order in which a wave hands out its instructions: at 128 values a head two
 // waves a SIMD keep the matrix unit at half of its rate. Measured, one causal sequence of
-// 16384, 16 heads on 4 of 128, bf16: d_q 1.45 ms (1.1 PFLOP/s), d_k and d_v 2.7 ms (1.0
-// PFLOP/s with S formed twice), delta 26 us.
+// 16384, 16 heads on 4 of 128, bf16, under the tracer: d_q 1.46 ms (1.1 PFLOP/s), d_k and
+// d_v 2.73 ms (1.0 PFLOP/s with S formed twice), δ 27 us; a call of them 4.09 ms.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -498,7 +499,8 @@ hipError_t bwd_go(const BwdArgs& a, hipStream_t stream) {
   p.tiles = int(tile_count(p.spans.tokens, 1, S::kBM, p.spans.sequences));
   const int blocks = p.tiles * p.kv_heads;
   ProfScope ps("dn_attention_dkv", stream);
-  // Apart too where the tiles of keys are too few to fill the CUs twice.
+  // Apart too where the tiles of keys are too few to fill the CUs twice (fp32, 1000 tokens,
+  // 6 heads on 2 of 40, 38 tiles: forward and gradients 211 us apart, 235 together).
   const bool both = p.d_k && p.d_v, apart = S::kApart || blocks < 2 * device_cu_count();
   hipLaunchKernelGGL((attention_dkv_kernel<T, HD>), dim3(unsigned(both && apart ? 2 * blocks : blocks)),
                      dim3(kNT), 0, stream, p, both && !apart ? -1 : p.d_k ? blocks : 0);

@@ -15,14 +15,18 @@
 // values take one wave each, the others four that meet in LDS (once for each of the
 // two chained means). The backward's workgroups walk rows with the next row's reads
 // in flight, and keep the column sums of their rows in registers: a second kernel
-// adds the workgroups' in order. Rows too long for registers are read again.
+// adds the workgroups' in order. Rows too long for registers are read again. In the
+// backward a part of what rows of 4097 to 8192 values need goes to scratch memory: 20
+// bytes a lane in bf16, 68 with fp32 weights, some 420 in fp32.
 //
 // Statistics, s before its rounding and all sums are fp32. As in add_rms_norm, the
 // forward normalises the unrounded s and the backward starts from the stored one (whose
 // rounding makes bf16 gradients 0.0024 off in the norm, where 0.0017 is their own).
 //
 // Measured, bf16: 32768 x 2048 with a gate a channel 101 us (5.3 TB/s, a copy's rate), its
-// gradient 168 us (4.8 TB/s) and 8 for the column sums; one row 3.5 us.
+// gradient 168 us (4.8 TB/s) and 8 for the column sums; one row 3.5 us. As many values in
+// wider rows, calls of the forward and the gradient in TB/s: 4096 columns 5.5 and 3.3, 8192
+// 5.0 and 3.6, 10000 3.4 and 1.5; in fp32 4.3 and 4.8, 4.1 and 2.0, 2.5 and 1.9.
 #include <algorithm>
 
 #include "gemm.hpp"
@@ -523,9 +527,11 @@ Shape shape_of(int64_t dim) {
 }
 
 // Workgroups of the backward: each walks rows and leaves one set of column sums. As many
-// as a CU has registers for at once (bf16 of up to 2048 values 152 a lane, fp32 up to
-// 191, longer rows more than 256): others would walk their rows alone, behind the rest
-// (32768 x 2048 in bf16: 218 us with four to a CU, 170 with three).
+// as a CU has registers for at once (bf16 of up to 2048 values 152 to 166 a lane, fp32 up
+// to 191, longer rows more than 256): others would walk their rows alone, behind the rest
+// (32768 x 2048 in bf16: 218 us with four to a CU, 170 with three). bf16 of up to 512
+// values with fp32 weights takes 174, of which two fit, not three: 48 us at 32768 x 512,
+// 41 with weights in bf16.
 int bwd_groups(int64_t rows, const Shape& s, int dtype) {
   const int64_t all = s.wpr == 1 ? (rows + 3) / 4 : rows;
   const int cu = s.nch == 0 ? 4 : s.nch > 1 ? 1 : dtype == DN_BF16 ? 3 : 2;

@@ -1,5 +1,5 @@
 // dn_embedding: out_i = scale · table[id_i]; dn_embedding_bwd: the table's gradient,
-// d_table[v] = scale · Σ d_out_i over the tokens i with id_i = v, added up in their
+// d_table[v] = scale · Σ d_out_i over the tokens i with id_i = v, added up in a fixed
 // order. An id that is not in [0, vocab), as padding has, stands for a row of zeros
 // and takes no part in the gradient.
 //
@@ -16,10 +16,10 @@
 //  2. Sums of 32 (8) consecutive sorted tokens each, however few or many share an id: a run
 //     that lies inside is written, one that crosses an end leaves its part in the
 //     workspace (fp32). Further workgroups write the rows that no token names.
-//  3. The parts of the runs that cross, in order.
+//  3. The parts of the runs that cross: four waves take every fourth, and meet in order.
 //
 // Measured, bf16, 16384 tokens as text has them, 50000 ids of 2048 values: lookup 26 us
-// (5.1 TB/s), sort 18, sums and zeros 66 (4.1 TB/s), join 10.
+// (5.1 TB/s), sort 18, sums and zeros 66 (4.1 TB/s), join 7.
 #include <algorithm>
 
 #include "gemm.hpp"

@@ -197,7 +197,8 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
 
 def embedding_backward(d_out: Tensor, tokens: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
     """The table's gradient [vocab, dim], of d_out's type: row v is scale times the sum
-    of d_out over the tokens with id v, summed in fp32 in the tokens' order."""
+    of d_out over the tokens with id v, summed in fp32 in a fixed order (not the tokens'):
+    two calls on one device agree to the bit."""
     ids = _ids(tokens)
     if d_out.dim() == 0 or d_out.shape[:-1] != tokens.shape:
         raise DeltaError(-2, f"d_out: expected {list(tokens.shape)} and a last axis, "
